@@ -756,7 +756,9 @@ std::vector<std::tuple<std::string, int64_t, int64_t, int64_t, int64_t>> bounds_
   using Reader = void (*)(msb::BoundsRecord*, bool);
   const std::pair<const char*, Reader> units[] = {{"nn", &msb::bounds_read_nn},
                                                   {"gemm", &msb::bounds_read_gemm},
-                                                  {"attention", &msb::bounds_read_attention}};
+                                                  {"attention", &msb::bounds_read_attention},
+                                                  {"logprob", &msb::bounds_read_logprob},
+                                                  {"embedding", &msb::bounds_read_embedding}};
   std::vector<std::tuple<std::string, int64_t, int64_t, int64_t, int64_t>> out;
   for (const auto& u : units) {
     msb::BoundsRecord r{};
@@ -767,7 +769,10 @@ std::vector<std::tuple<std::string, int64_t, int64_t, int64_t, int64_t>> bounds_
   return out;
 }
 
+void register_token_ops(pybind11::module_& mod);  // bindings_token_ops.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
+  register_token_ops(mod);
   mod.doc() = "minispeed_b200 sm_100a kernels";
   mod.def("grad_stats", &grad_stats);
   mod.def("stats_finalize", &stats_finalize);

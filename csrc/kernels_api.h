@@ -31,7 +31,8 @@ enum BoundsSite : int {
   kSiteGemmSlot = 5,        // split-K / stream-K partial beyond the workspace
   kSiteGemmCounter = 6,     // stream-K / fixup tile counter beyond the counter array
   kSiteGemmColsum = 7,      // dGELU column-sum partial beyond [ceil(M / 32), N]
-  kSiteCount = 8
+  kSiteLogprobToken = 8,    // token of a log probability outside [0, V), not ignore_index
+  kSiteCount = 9
 };
 struct BoundsRecord {
   unsigned long long count;
@@ -42,6 +43,8 @@ bool bounds_check_build();
 void bounds_read_nn(BoundsRecord* out, bool reset);
 void bounds_read_gemm(BoundsRecord* out, bool reset);
 void bounds_read_attention(BoundsRecord* out, bool reset);
+void bounds_read_logprob(BoundsRecord* out, bool reset);
+void bounds_read_embedding(BoundsRecord* out, bool reset);
 
 // ---- step pipeline (step_kernels.cu)
 int grad_stats(const void* x, int dtype, long long n, float mul, float* partials,
@@ -109,6 +112,34 @@ void embedding_fwd(const long long* idx, const void* wte, const void* wpe, void*
 void embedding_bwd(const void* dout, const long long* idx, float* acc, unsigned char* touched,
                    void* dwte, int acc_wte, void* dwpe, int acc_wpe, long long M, int T_len,
                    int C, long long V, int dtype, cudaStream_t st);
+// log probabilities of tokens (logprob_kernels.cu): stats [M, 3] is what the
+// backward needs of a row; entropy and the top_* may be null (k = 0)
+void logprob_fwd(const void* logits, long long ld, const long long* tok, long long M, int V,
+                 float temperature, long long ignore_index, int k, float* logp, float* entropy,
+                 float* top_logp, long long* top_tok, float* stats, int dtype, cudaStream_t st);
+void logprob_bwd(const void* logits, long long ld, const long long* tok, long long M, int V,
+                 float temperature, long long ignore_index, int k, const long long* top_tok,
+                 const float* stats, const float* g_logp, const float* g_ent, const float* g_top,
+                 void* dx, long long ld_dx, int dtype, cudaStream_t st);
+// embedding with scaling (embedding_sorted.cu); the backward writes the rows of
+// the tokens that occur (grad is zero elsewhere already) or adds to them, and
+// needs scaled_embedding_ws words of scratch; padding < 0: none
+void scaled_embedding_fwd(const long long* idx, const void* w, void* out, long long n, int C,
+                          long long V, float scale, int dtype, cudaStream_t st);
+long long scaled_embedding_ws(long long n, int C);
+void scaled_embedding_bwd(const void* dout, const long long* idx, void* grad, bool accumulate,
+                          unsigned* ws, long long n, int C, long long V, long long padding,
+                          float scale, int dtype, cudaStream_t st);
+// activations in 8 bits (pack8_kernels.cu): codes [rows, 32 * nb], scales [rows, nb],
+// nb = ceil(D / 32); swiglu8_*: rows of [gate (F) | up (F)], packed as 2 * rows rows of F
+void pack8(const void* x, long long ld, signed char* codes, unsigned char* scales, long long rows,
+           int D, int dtype, cudaStream_t st);
+void unpack8(const signed char* codes, const unsigned char* scales, void* x, long long rows, int D,
+             int dtype, cudaStream_t st);
+void swiglu8_fwd(const void* gu, void* h, signed char* codes, unsigned char* scales,
+                 long long rows, int F, int dtype, cudaStream_t st);
+void swiglu8_bwd(const void* dh, const signed char* codes, const unsigned char* scales, void* dgu,
+                 long long rows, int F, int dtype, cudaStream_t st);
 void rope(void* x, const float* cos_t, const float* sin_t, long long BT, int T_len, int H, int D,
           long long row_stride, bool inverse, int dtype, cudaStream_t st);
 

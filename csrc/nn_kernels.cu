@@ -25,86 +25,10 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "vec.cuh"
 
 namespace msb {
 namespace {
-
-template <typename T>
-struct alignas(16) Pack8 {
-  T v[8];
-};
-
-// 2^x on the special-function unit; e^x = 2^(x * log2(e))
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// 8-element accesses: one 16-byte transaction when the address allows it,
-// element-wise otherwise.  Parameters are views into a flat arena at
-// arbitrary element offsets, so weights and biases need not be aligned.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
-  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-    Pack8<T> r = *reinterpret_cast<const Pack8<T>*>(p);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = to_f32(r.v[k]);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = to_f32(p[k]);
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
-  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-    Pack8<T> r;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) r.v[k] = from_f32<T>(f[k]);
-    *reinterpret_cast<Pack8<T>*>(p) = r;
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) p[k] = from_f32<T>(f[k]);
-  }
-}
-
-// 8 16-bit values as one 16-byte quad of registers, unpacked and packed two
-// at a time (a bf16 is the upper half of an fp32; element 0 is the low half
-// of the first word), so packed rows take 4 registers per 8 values.
-template <typename T>
-__device__ __forceinline__ void unpack_u4(const uint4& r, float (&f)[8]) {
-  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-      f[2 * q] = __uint_as_float(w[q] << 16);
-      f[2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
-    } else {
-      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[q]));
-      f[2 * q] = v.x;
-      f[2 * q + 1] = v.y;
-    }
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ uint4 pack_u4(const float (&f)[8]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * q], f[2 * q + 1]);
-      w[q] = *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-      const __half2 h = __floats2half2_rn(f[2 * q], f[2 * q + 1]);
-      w[q] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
 
 // ------------------------------------------------------------ layernorm
 // One warp per row; the row stays in registers (NV vectors of 8 per lane).

@@ -37,6 +37,7 @@ class GPTConfig:
     n_embd: int = 768
     activation_checkpointing: bool = False
     ln_eps: float = 1e-5
+    checkpoint_bits: Optional[int] = None   # 8: checkpointed blocks keep their inputs in 8 bits
 
 
 def gpt2_small(**kw) -> GPTConfig:
@@ -101,8 +102,13 @@ class GPT(nn.Module):
         self.head = nn.Linear(cfg.n_embd, cfg.vocab_size, bias=False)
         self.head.weight = self.wte.weight
 
-    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None):
-        """Logits [B, T, V] or, with ``targets``, the mean cross-entropy loss."""
+    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None,
+                logprobs: Optional[dict] = None):
+        """Logits [B, T, V] or, with ``targets``, the mean cross-entropy loss.
+
+        With ``targets`` and ``logprobs``, a dict of
+        :func:`~minispeed_b200.ops.nn.token_logprobs` options (it may be empty),
+        the log probabilities of the targets instead of their mean loss."""
         B, T = idx.shape
         if T > self.block_size:
             raise ValueError(f"sequence length {T} > block_size {self.block_size}")
@@ -111,13 +117,15 @@ class GPT(nn.Module):
         delta = None
         for blk in self.blocks:
             if self.config.activation_checkpointing and self.training and torch.is_grad_enabled():
-                x, delta = checkpoint(blk, x, delta)
+                x, delta = checkpoint(blk, x, delta, save_bits=self.config.checkpoint_bits)
             else:
                 x, delta = blk(x, delta)
         _, h = ops.add_norm(x, delta, self.ln_f.weight, self.ln_f.bias, self.config.ln_eps)
         logits = ops.linear(h, self.head.weight, pad_out=64)
         if targets is None:
             return logits
+        if logprobs is not None:
+            return ops.token_logprobs(logits, targets, **logprobs)
         return ops.cross_entropy(logits, targets)
 
     def num_params(self) -> int:

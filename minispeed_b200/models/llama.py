@@ -39,6 +39,11 @@ class LlamaConfig:
     rope_theta: float = 500000.0
     norm_eps: float = 1e-5
     activation_checkpointing: bool = False
+    checkpoint_bits: Optional[int] = None    # 8: checkpointed blocks keep their inputs in 8 bits
+    swiglu_save_bits: Optional[int] = None   # 8: SwiGLU keeps its input for backward in 8 bits
+    # embeddings times this number; their gradient is then summed by sorted
+    # tokens (the same from run to run, and without an fp32 [V, C] accumulator)
+    embed_scale: Optional[float] = None
 
 
 def llama3_8b(**kw) -> LlamaConfig:
@@ -74,9 +79,11 @@ class FeedForward(nn.Module):
         super().__init__()
         self.gate_up = nn.Linear(cfg.n_embd, 2 * cfg.ffn_hidden, bias=False)
         self.down = nn.Linear(cfg.ffn_hidden, cfg.n_embd, bias=False)
+        self.save_bits = cfg.swiglu_save_bits
 
     def forward(self, h):
-        return ops.linear(ops.swiglu(ops.linear(h, self.gate_up.weight)), self.down.weight)
+        gu = ops.linear(h, self.gate_up.weight)
+        return ops.linear(ops.swiglu(gu, self.save_bits), self.down.weight)
 
 
 class LlamaBlock(nn.Module):
@@ -115,20 +122,28 @@ class Llama(nn.Module):
                                          self.config.rope_theta, device)
         return self._rope
 
-    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None):
+    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None,
+                logprobs: Optional[dict] = None):
+        """Logits, mean loss or the targets' log probabilities, as ``GPT.forward``."""
         B, T = idx.shape
         cos, sin = self._tables(T, idx.device)
-        x = ops.embedding(idx, self.embed.weight)
+        if self.config.embed_scale is None:
+            x = ops.embedding(idx, self.embed.weight)
+        else:
+            x = ops.scaled_embedding(idx, self.embed.weight, self.config.embed_scale)
         delta = None
         for blk in self.blocks:
             if self.config.activation_checkpointing and self.training and torch.is_grad_enabled():
-                x, delta = checkpoint(blk, x, delta, cos, sin)
+                x, delta = checkpoint(blk, x, delta, cos, sin,
+                                      save_bits=self.config.checkpoint_bits)
             else:
                 x, delta = blk(x, delta, cos, sin)
         _, h = ops.add_norm(x, delta, self.norm.weight, None, self.config.norm_eps, rms=True)
         logits = ops.linear(h, self.head.weight, pad_out=64)
         if targets is None:
             return logits
+        if logprobs is not None:
+            return ops.token_logprobs(logits, targets, **logprobs)
         return ops.cross_entropy(logits, targets)
 
 

@@ -32,6 +32,7 @@ BOUNDS_SITES = {
     5: "GEMM partial beyond the workspace",
     6: "GEMM tile counter beyond the counter array",
     7: "GEMM column-sum partial beyond its buffer",
+    8: "log-probability token outside [0, V)",
 }
 
 

@@ -10,9 +10,14 @@ Ops:
   ``norm``            LayerNorm/RMSNorm without a residual
   ``linear``          x @ W^T + b through :mod:`.gemm`
   ``linear_gelu``     gelu(x @ W^T + b) (exact erf GELU, saves the pre-activation)
-  ``swiglu``          silu(gate) * up on a fused [gate | up] projection
+  ``swiglu``          silu(gate) * up on a fused [gate | up] projection; can keep its
+                      input in 8 bits for backward
+  ``pack_activation`` a tensor in 8 bits with a scale per 32 values, and back
   ``cross_entropy``   fused softmax cross-entropy on model-dtype logits
+  ``token_logprobs``  log probabilities of given tokens, entropy, top alternatives
   ``embedding``       token (+ learned position) embedding
+  ``scaled_embedding`` token embedding times a scale; its gradient summed in a
+                      fixed order, by sorted tokens
   ``rope_``           rotary embedding on q/k views
 
 Reference: the layers of the example model (``examples/train_lm.py:62-115``:
@@ -26,7 +31,8 @@ from __future__ import annotations
 
 import math
 from contextlib import contextmanager
-from typing import Optional, Tuple
+from dataclasses import dataclass
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -420,12 +426,141 @@ class _SwiGLU(torch.autograd.Function):
         return dgu
 
 
-def swiglu(gu: torch.Tensor) -> torch.Tensor:
-    """``silu(gu[..., :F]) * gu[..., F:]`` for a fused gate/up projection."""
-    if gu.is_cuda:
-        return _SwiGLU.apply(gu.contiguous())
+class _SwiGLU8(torch.autograd.Function):
+    """SwiGLU that saves its input packed: the forward kernel writes the codes
+    in the pass that computes ``h``, the backward kernel reads them in place of
+    the input."""
+
+    @staticmethod
+    def forward(ctx, gu):
+        ctx.set_materialize_grads(False)
+        if gu.is_cuda:
+            h, codes, scales = _C().swiglu8_fwd(gu, True)
+        else:
+            F_ = gu.shape[-1] // 2
+            codes, scales = _pack8_torch(gu.reshape(-1, F_))
+            h = _swiglu_torch(gu)
+        ctx.save_for_backward(codes, scales)
+        return h
+
+    @staticmethod
+    def backward(ctx, dh):
+        if dh is None:
+            return None
+        codes, scales = ctx.saved_tensors
+        if dh.is_cuda:
+            return _C().swiglu8_bwd(dh.contiguous(), codes, scales)
+        F_ = dh.shape[-1]
+        g, u = _unpack8_torch(codes, scales, F_).view(-1, 2, F_).unbind(1)
+        d = dh.reshape(-1, F_).float()
+        s = torch.sigmoid(g)
+        dgu = torch.cat([d * u * s * (1 + g * (1 - s)), d * g * s], -1)
+        return dgu.view(*dh.shape[:-1], 2 * F_).to(dh.dtype)
+
+
+def _swiglu_torch(gu: torch.Tensor) -> torch.Tensor:
     g, u = gu.chunk(2, dim=-1)
     return (F.silu(g.float()) * u.float()).to(gu.dtype)
+
+
+def _check_save_bits(save_bits) -> bool:
+    """True for 8-bit saves, False for saves as they are (None)."""
+    if save_bits not in (None, 8):
+        raise ValueError(f"save_bits must be None or 8, got {save_bits!r}")
+    return save_bits == 8
+
+
+def swiglu(gu: torch.Tensor, save_bits: Optional[int] = None) -> torch.Tensor:
+    """``silu(gu[..., :F]) * gu[..., F:]`` for a fused gate/up projection.
+
+    ``save_bits=8`` keeps ``gu`` for backward in 8 bits (the format of
+    :func:`pack_activation`, gate and up in blocks of their own): about half
+    the memory of a 16-bit ``gu``.  The output is that of the exact input;
+    the gradient is the formula's at the packed values."""
+    if _check_save_bits(save_bits):
+        _check_packable(gu)
+        if gu.shape[-1] % 2:
+            raise ValueError(f"swiglu: the last axis holds [gate | up], got width {gu.shape[-1]}")
+        if gu.numel() and torch.is_grad_enabled() and gu.requires_grad:
+            return _SwiGLU8.apply(gu.contiguous())
+        if gu.numel() and gu.is_cuda:
+            return _C().swiglu8_fwd(gu.contiguous(), False)[0]
+        return _swiglu_torch(gu)
+    if gu.is_cuda:
+        return _SwiGLU.apply(gu.contiguous())
+    return _swiglu_torch(gu)
+
+
+# ---------------------------------------------------- 8-bit activations
+PACK_BLOCK = 32   # values per scale
+
+_DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _check_packable(x: torch.Tensor) -> None:
+    if x.dtype not in _DTYPE_CODES:
+        raise TypeError(f"8-bit activations: fp32, fp16 or bf16 tensors, got {x.dtype}")
+    if x.dim() == 0:
+        raise ValueError("8-bit activations: a tensor with at least one axis is needed")
+
+
+def _pack8_torch(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Codes [rows, 32 * blocks] and scale bytes [rows, blocks] of a matrix."""
+    f = F.pad(x.detach().float(), (0, -x.shape[-1] % PACK_BLOCK)).unflatten(-1, (-1, PACK_BLOCK))
+    field = (f.view(torch.int32) & 0x7FFFFFFF).amax(-1, keepdim=True) >> 23
+    b = torch.where(field == 255, field, (field - 6).clamp(min=0))
+    q = torch.round(torch.ldexp(f, 127 - b)).clamp(-127, 127)
+    q = torch.where(b == 255, 0.0, q)
+    return q.to(torch.int8).flatten(-2), b.squeeze(-1).to(torch.uint8)
+
+
+def _unpack8_torch(codes: torch.Tensor, scales: torch.Tensor, width: int) -> torch.Tensor:
+    b = scales[..., None].int()
+    f = torch.ldexp(codes.unflatten(-1, (-1, PACK_BLOCK)).float(), b - 127)
+    return torch.where(b == 255, float("nan"), f).flatten(-2)[..., :width]
+
+
+@dataclass(frozen=True)
+class PackedActivation:
+    """A tensor held in 8 bits: one signed byte a value and one byte, the
+    exponent of a power-of-two scale, for every 32 values of the last axis (the
+    last block of a row may be short)."""
+
+    codes: torch.Tensor        # int8 [rows, 32 * blocks]
+    scales: torch.Tensor       # uint8 [rows, blocks]
+    shape: torch.Size
+    dtype: torch.dtype
+
+    def unpack(self) -> torch.Tensor:
+        """The tensor again, contiguous, in its own type.  Values are off by at
+        most half a step of their block's scale, 2^-7 of its largest magnitude
+        (a whole step for values that round to 128 steps); a block that held an
+        infinity or a NaN is all NaN."""
+        if not self.scales.numel():
+            return torch.empty(self.shape, dtype=self.dtype, device=self.codes.device)
+        if self.codes.is_cuda:
+            x = _C().unpack8(self.codes, self.scales, self.shape[-1], _DTYPE_CODES[self.dtype])
+        else:
+            x = _unpack8_torch(self.codes, self.scales, self.shape[-1]).to(self.dtype)
+        return x.view(self.shape)
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.nbytes + self.scales.nbytes
+
+
+def pack_activation(x: torch.Tensor) -> PackedActivation:
+    """``x`` (fp32, fp16 or bf16, any shape with at least one axis) in 8 bits;
+    :meth:`PackedActivation.unpack` brings it back.  No gradient flows through
+    the pair: it is for what a backward pass keeps."""
+    _check_packable(x)
+    x = x.detach()
+    if not x.numel():
+        empty = x.new_empty((0, 0), dtype=torch.uint8)
+        return PackedActivation(empty.view(torch.int8), empty, x.shape, x.dtype)
+    x2 = as_matrix(x, x.shape[-1])
+    codes, scales = _C().pack8(x2) if x.is_cuda else _pack8_torch(x2)
+    return PackedActivation(codes, scales, x.shape, x.dtype)
 
 
 # -------------------------------------------------------- cross entropy
@@ -500,6 +635,120 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int
                            ignore_index=ignore_index)
 
 
+# ------------------------------------------------- token log probabilities
+MAX_TOP_K = 32
+
+
+class TokenLogprobs(NamedTuple):
+    """What :func:`token_logprobs` returns; what was not asked for is None."""
+
+    logprobs: torch.Tensor                 # fp32, the tokens' shape
+    entropy: Optional[torch.Tensor]        # fp32, the tokens' shape
+    top_logprobs: Optional[torch.Tensor]   # fp32 [..., k], most probable first
+    top_tokens: Optional[torch.Tensor]     # int64 [..., k]
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, temperature, entropy, top_k, ignore_index):
+        ctx.set_materialize_grads(False)
+        l2 = as_matrix(logits, logits.shape[-1])
+        t = tokens.reshape(-1).contiguous()
+        lp, ent, top_lp, top, stats = _C().logprob_fwd(l2, t, temperature, entropy, top_k,
+                                                       ignore_index)
+        ctx.save_for_backward(l2, t, top, stats)
+        ctx.shape = logits.shape
+        ctx.args = (temperature, ignore_index)
+        shape = tokens.shape
+        if top is not None:
+            top_lp, top = top_lp.view(*shape, top_k), top.view(*shape, top_k)
+            ctx.mark_non_differentiable(top)
+        return lp.view(shape), None if ent is None else ent.view(shape), top_lp, top
+
+    @staticmethod
+    def backward(ctx, g_lp, g_ent, g_top, _):
+        if g_lp is None and g_ent is None and g_top is None:
+            return (None,) * 6
+        l2, t, top, stats = ctx.saved_tensors
+        dx = _C().logprob_bwd(l2, t, top, stats, g_lp, g_ent, g_top, *ctx.args)
+        return (dx.view(ctx.shape),) + (None,) * 5
+
+
+def _token_logprobs_torch(logits, tokens, temperature, entropy, top_k, ignore_index):
+    """The same in PyTorch operations."""
+    keep = tokens != ignore_index
+    at = torch.where(keep, tokens, 0)
+    if bool(((at < 0) | (at >= logits.shape[-1])).any()):
+        raise IndexError("token_logprobs: token outside the vocabulary")
+    x = logits.float()
+    empty = (x == -math.inf).all(-1, keepdim=True)
+    # an empty row is computed as a row of zeros, and replaced below; the largest
+    # logit is subtracted first: dividing the lowest value of fp32 overflows
+    x = torch.where(empty, 0.0, x)
+    logp = torch.log_softmax((x - x.detach().amax(-1, keepdim=True)) / temperature, -1)
+    keep_row, empty_row = keep[..., None], empty[..., 0]
+
+    def settle(v, k, e, of_empty):
+        return torch.where(k, torch.where(e, of_empty, v), 0.0)
+
+    lp = settle(logp.gather(-1, at[..., None])[..., 0], keep, empty_row, -math.inf)
+    ent = top_lp = top = None
+    if entropy:
+        # p log p is zero where p is, in its gradient too
+        live = torch.where(logp == -math.inf, 0.0, logp)
+        ent = settle(-(logp.exp() * live).sum(-1), keep, empty_row, 0.0)
+    if top_k:
+        top = torch.sort(logits.detach(), dim=-1, descending=True, stable=True).indices[..., :top_k]
+        top_lp = settle(logp.gather(-1, top), keep_row, empty, -math.inf)
+        top = torch.where(keep_row, top, -1)
+    return lp, ent, top_lp, top
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 1.0,
+                   entropy: bool = False, top_k: int = 0, ignore_index: int = -100
+                   ) -> TokenLogprobs:
+    """Log probabilities of ``tokens`` under softmax(``logits`` / ``temperature``).
+
+    ``logits`` [..., V] in fp32, fp16 or bf16 (rows may be padded, as
+    ``linear(pad_out=)`` leaves them) and int64 ``tokens`` [...].  All results
+    are fp32 and computed in fp32.  ``entropy`` adds the entropy of every
+    position, ``top_k`` (at most 32) its most probable tokens and their log
+    probabilities: by logit, the lower index first among equals.
+
+    Positions whose token is ``ignore_index`` are skipped: their results are 0
+    (top tokens -1), their gradient is zero.  A logit of -inf excludes a token;
+    a position where every logit is -inf has log probabilities -inf and no
+    entropy or gradient, and one with a NaN or +inf is NaN throughout (its top
+    tokens are then unspecified, within the vocabulary).  A token outside the
+    vocabulary raises ``IndexError`` on the CPU; on CUDA, where raising would
+    need a synchronization, its log probability is NaN and has no gradient.
+
+    Gradients flow to ``logits`` from the log probabilities, the entropy and
+    the top log probabilities.  Unlike :func:`cross_entropy` this leaves the
+    logits as they are."""
+    if logits.dtype not in _DTYPE_CODES:
+        raise TypeError(f"token_logprobs: fp32, fp16 or bf16 logits, got {logits.dtype}")
+    if tokens.dtype != torch.int64:
+        raise TypeError(f"token_logprobs: int64 tokens, got {tokens.dtype}")
+    if logits.dim() == 0 or tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"token_logprobs: logits {tuple(logits.shape)} need tokens "
+                         f"{tuple(logits.shape[:-1])}, got {tuple(tokens.shape)}")
+    if tokens.device != logits.device:
+        raise ValueError(f"token_logprobs: logits on {logits.device}, tokens on {tokens.device}")
+    V = logits.shape[-1]
+    if V == 0:
+        raise ValueError("token_logprobs: the vocabulary is empty")
+    if not 0 <= top_k <= min(MAX_TOP_K, V):
+        raise ValueError(f"token_logprobs: top_k must be between 0 and {min(MAX_TOP_K, V)}, "
+                         f"got {top_k}")
+    if not (math.isfinite(temperature) and temperature > 0):
+        raise ValueError(f"token_logprobs: temperature must be positive, got {temperature}")
+    args = (float(temperature), bool(entropy), int(top_k), int(ignore_index))
+    if logits.is_cuda and logits.numel():
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, *args))
+    return TokenLogprobs(*_token_logprobs_torch(logits, tokens, *args))
+
+
 # ------------------------------------------------------------ embedding
 class _Embedding(torch.autograd.Function):
     @staticmethod
@@ -563,6 +812,66 @@ def embedding(idx: torch.Tensor, wte: torch.Tensor, wpe: Optional[torch.Tensor] 
     if wpe is not None:
         x = x + wpe[: idx.shape[1]]
     return x
+
+
+class _ScaledEmbedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, idx, weight, scale, padding):
+        idx = idx.contiguous()
+        if weight.is_cuda:
+            out = _C().scaled_embedding_fwd(idx, weight.contiguous(), scale)
+        else:
+            out = (F.embedding(idx, weight).float() * scale).to(weight.dtype)
+        ctx.save_for_backward(idx)
+        ctx.weight = weight
+        ctx.args = (weight.shape[0], padding, scale)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        (idx,) = ctx.saved_tensors
+        V, padding, scale = ctx.args
+        sink = grad_sink(ctx.weight)
+        if dout.is_cuda:
+            dw = _C().scaled_embedding_bwd(dout.contiguous(), idx, V, padding, scale, sink)
+            return None, None if sink is not None else dw, None, None
+        rows = dout.reshape(idx.numel(), -1).float() * scale
+        rows = torch.where((idx.reshape(-1) == padding)[:, None], 0.0, rows)
+        dw = torch.zeros(V, dout.shape[-1]).index_add_(0, idx.reshape(-1), rows)
+        return None, dw.to(dout.dtype), None, None
+
+
+def scaled_embedding(idx: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
+                     padding_idx: Optional[int] = None) -> torch.Tensor:
+    """``weight[idx] * scale`` for int64 ``idx`` of any shape and a [V, C] table.
+
+    The gradient of a row is the fp32 sum over its positions in ascending
+    order, rounded once, whatever runs beside it: the same from run to run
+    (:func:`embedding` adds with atomics, and keeps an fp32 [V, C] accumulator,
+    which this does not).  It goes into ``weight.grad`` where the engine has
+    bound one.  Positions equal to ``padding_idx`` give no gradient.
+
+    A token outside the table raises ``IndexError`` on the CPU; on CUDA it
+    reads as a zero row and gives no gradient, as in :func:`embedding`."""
+    if idx.dtype != torch.int64:
+        raise TypeError(f"scaled_embedding: int64 tokens, got {idx.dtype}")
+    if weight.dtype not in _DTYPE_CODES:
+        raise TypeError(f"scaled_embedding: an fp32, fp16 or bf16 table, got {weight.dtype}")
+    if weight.dim() != 2 or not weight.numel():
+        raise ValueError(f"scaled_embedding: the table must be [V, C] and not empty, got "
+                         f"{tuple(weight.shape)}")
+    if idx.device != weight.device:
+        raise ValueError(f"scaled_embedding: tokens on {idx.device}, table on {weight.device}")
+    if not math.isfinite(scale):
+        raise ValueError(f"scaled_embedding: scale must be finite, got {scale}")
+    V = weight.shape[0]
+    padding = -1
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
+            raise ValueError(f"scaled_embedding: padding_idx {padding_idx} outside a table of "
+                             f"{V} rows")
+        padding = padding_idx % V
+    return _ScaledEmbedding.apply(idx, weight, float(scale), padding)
 
 
 # ------------------------------------------------------------------ rope
