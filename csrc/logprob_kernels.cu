@@ -1,7 +1,7 @@
 // Log probabilities of given tokens, with the entropy of every position and
 // its most probable alternatives, over model-dtype logits; and their gradient.
 //
-// Row x[0..V), temperature T, c = log2(e) / T, m = max(x), z_i = (x_i - m) c:
+// Row x[0..V), temperature T, c = log2(e) / T, m = max(x), z_i = x_i c - m c:
 //
 //   s = sum 2^z_i      t = sum 2^z_i z_i
 //   log p_i = ln 2 (z_i - log2 s)        H = ln 2 (log2 s - t / s)
@@ -14,6 +14,8 @@
 // A logit of -inf has probability zero and adds nothing anywhere; a row with
 // nothing else is empty: its log probabilities are -inf, its entropy and its
 // gradient zero.  A NaN or +inf in a row makes all its values NaN.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "vec.cuh"
 
@@ -23,195 +25,570 @@ MSB_BOUNDS_TU(logprob)
 
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kThreads = 512;
+constexpr int kMaxK = 32;
+constexpr int kMaxCluster = 8;
+constexpr int kGroups = 64;    // groups of threads whose maxima give a threshold, >= kMaxK
+constexpr int kCand = 1024;    // candidates kept above the threshold, and
+constexpr int kEqual = 512;    // at it
+static_assert(kMaxK <= kGroups && kMaxK + kEqual <= kCand && kMaxCluster * kMaxK <= kCand, "");
+
+// 16 bytes of logits
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  uint4 r;
+  __device__ __forceinline__ void unpack(float (&f)[N]) const {
+    if constexpr (sizeof(T) == 2) {
+      unpack_u4<T>(r, f);
+    } else {
+      f[0] = __uint_as_float(r.x);
+      f[1] = __uint_as_float(r.y);
+      f[2] = __uint_as_float(r.z);
+      f[3] = __uint_as_float(r.w);
+    }
+  }
+  // the largest value that is no NaN (a NaN where all are); two at a time in 16 bits
+  __device__ __forceinline__ float max() const {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&r);
+      const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+      return fmaxf(__low2float(m), __high2float(m));
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2* p = reinterpret_cast<const __half2*>(&r);
+      const __half2 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+      return fmaxf(__low2float(m), __high2float(m));
+    } else {
+      return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)),
+                   fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+    }
+  }
+  // -inf everywhere: adds nothing
+  __device__ __forceinline__ void clear() {
+    const unsigned w = sizeof(T) == 4 ? 0xff800000u
+                       : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+    r = make_uint4(w, w, w, w);
+  }
+};
 
 // (value, index) as one number: larger value first, then the lower index.
 // NaN has no place in the order (0).
-__device__ __forceinline__ unsigned long long key_of(float v, int i) {
-  if (v != v) return 0ull;
+__device__ __forceinline__ unsigned order_of(float v) {
   const int b = __float_as_int(v + 0.f);  // -0 counts as 0
-  const unsigned u = b < 0 ? ~(unsigned)b : (unsigned)b | 0x80000000u;
-  return ((unsigned long long)u << 32) | (0xffffffffu - (unsigned)i);
+  return b < 0 ? ~(unsigned)b : (unsigned)b | 0x80000000u;
+}
+__device__ __forceinline__ unsigned long long key_of(float v, int i) {
+  return v != v ? 0ull : ((unsigned long long)order_of(v) << 32) | (0xffffffffu - (unsigned)i);
 }
 __device__ __forceinline__ int key_index(unsigned long long k) {
   return (int)(0xffffffffu - (unsigned)k);
 }
 
-__device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = w > v ? w : v;
-  }
-  return v;
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
 
-// running maximum m of the logits, and the sums s, t relative to it.  The
-// difference of two logits is taken before it is scaled: the lowest value of
-// fp32 or bf16, a common mask, times c overflows.
+// The exponents of a row are z = x c - m c, one fused operation on the rounded
+// product m c (the same one wherever the row's z are computed, so its rounding
+// cancels).  Where m c comes near fp32's range (the lowest value of fp32 or bf16
+// is a common mask) the row is `wide` and z = (x - m) c.
+__device__ __forceinline__ bool is_wide(float m, float c) {
+  return fabsf(m * c) >= 1e37f && m != -INFINITY;
+}
+__device__ __forceinline__ float reference(float m, float c) {   // of -inf: 0
+  return m == -INFINITY ? 0.f : fminf(fmaxf(m * c, -1e37f), 1e37f);
+}
+
+// exponents at or under this give 2^z = 0; a larger one in z's place keeps
+// 0 * z a number
+constexpr float kLowZ = -200.f;
+
+// a thread's running maximum, its reference, and the sums relative to it
 struct Sums {
-  float m, s, t;
+  float m = -INFINITY, ref = 0.f, s = 0.f, t = 0.f;
+  // to a reference above; from that of nothing yet (0) to any
+  __device__ __forceinline__ void rebase(float to) {
+    const float d = fminf(fmaxf(ref - to, kLowZ), 0.f), f = ex2_approx(d);
+    t = f * (t + s * d);
+    s *= f;
+    ref = to;
+  }
 };
-// weight of a sum whose maximum lies d below the new one
-__device__ __forceinline__ void scale_down(float& s, float& t, float d) {
-  const float f = ex2_approx(d);
-  t = f == 0.f ? 0.f : f * (t + s * d);
-  s *= f;
+
+template <bool ENT>
+__device__ __forceinline__ void add_z(float z, float& s, float& t) {
+  if (ENT) z = max_nan(z, kLowZ);
+  const float e = ex2_approx(z);
+  s += e;
+  if (ENT) t = fmaf(e, z, t);
 }
-__device__ __forceinline__ void add(Sums& a, float x, float c) {
-  if (x > a.m) {
-    if (a.m != -INFINITY) scale_down(a.s, a.t, (a.m - x) * c);
-    a.s += 1.f;
-    a.m = x;
-  } else if (x != -INFINITY) {  // NaN as well
-    const float z = (x - a.m) * c, e = ex2_approx(z);
-    a.s += e;
-    a.t += e == 0.f ? 0.f : e * z;
+
+template <typename T, bool ENT>
+__device__ __forceinline__ void add_vec(Sums& a, const Vec<T>& v, float c) {
+  constexpr int N = Vec<T>::N;
+  const float m = v.max();
+  if (m > a.m) {
+    a.rebase(reference(m, c));
+    a.m = m;
   }
-}
-__device__ __forceinline__ Sums merge(Sums a, Sums b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  if (a.m != -INFINITY) scale_down(a.s, a.t, (a.m - m) * c);
-  if (b.m != -INFINITY) scale_down(b.s, b.t, (b.m - m) * c);
-  return {m, a.s + b.s, a.t + b.t};
-}
-__device__ __forceinline__ Sums warp_merge(Sums v, float c) {
+  float x[N], s1 = 0.f, t1 = 0.f;
+  v.unpack(x);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Sums w = {__shfl_xor_sync(0xffffffffu, v.m, o), __shfl_xor_sync(0xffffffffu, v.s, o),
-                    __shfl_xor_sync(0xffffffffu, v.t, o)};
-    v = merge(v, w, c);
+  for (int k = 0; k < N; k += 2) {
+    add_z<ENT>(fmaf(x[k], c, -a.ref), a.s, a.t);
+    add_z<ENT>(fmaf(x[k + 1], c, -a.ref), s1, t1);
   }
+  a.s += s1;
+  a.t += t1;
+}
+
+template <bool ENT>
+__device__ __forceinline__ void add_one(Sums& a, float x, float c) {
+  if (x > a.m) {
+    a.rebase(reference(x, c));
+    a.m = x;
+  }
+  add_z<ENT>(fmaf(x, c, -a.ref), a.s, a.t);
+}
+
+// The part of a row that a block of the cluster reads: vectors [v0, v1) of the
+// row's aligned middle; the first block also has the `head` values before it,
+// the last the `tail` behind it.
+template <typename T>
+struct Part {
+  const T* row;
+  const uint4* mid;
+  int head, tail, nv, v0, v1, V;
+  bool first, last;
+  __device__ Part(const T* row_, int V_, unsigned q, unsigned R) : row(row_), V(V_) {
+    constexpr int N = Vec<T>::N;
+    const int off = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T);
+    head = min(off, V);
+    nv = (V - head) / N;
+    tail = V - head - nv * N;
+    mid = reinterpret_cast<const uint4*>(row + head);
+    const int per = (nv + (int)R - 1) / (int)R;
+    v0 = min(nv, per * (int)q);
+    v1 = min(nv, v0 + per);
+    first = q == 0;
+    last = q == R - 1;
+  }
+  // index of a vector's first value
+  __device__ __forceinline__ int at(int v) const { return head + v * Vec<T>::N; }
+  // number of this block's values outside vectors, and the index of one
+  __device__ __forceinline__ int loose() const { return (first ? head : 0) + (last ? tail : 0); }
+  __device__ __forceinline__ int loose_at(int i) const {
+    return first && i < head ? i : V - tail + i - (first ? head : 0);
+  }
+};
+
+template <typename F>
+__device__ __forceinline__ float block_reduce(float v, float* buf, F&& f) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = buf[threadIdx.x & (kThreads / 32 - 1)];
+#pragma unroll
+  for (int o = kThreads / 64; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 
-// One block a row: one pass for the sums, k more for the k alternatives.
+// What a block knows of its part of the row, read by the cluster's first block.
+struct alignas(8) Shared {
+  unsigned long long best[kMaxK];      // its alternatives, best first; 0: none
+  unsigned long long cand[kCand];
+  unsigned long long equal[kEqual];
+  unsigned long long round[kThreads / 32];
+  float ms[3];                         // maximum, s, t
+  float buf[3][kThreads / 32];
+  float thread_max[kThreads];
+  unsigned group[kGroups];
+  unsigned short winner[kThreads];
+  float threshold;
+  int winners, above, at;
+};
+
+// The k best of `n` keys in order, by counting for each how many beat it.
+__device__ __forceinline__ void rank_keys(const unsigned long long* keys, int n,
+                                          unsigned long long* out, int k) {
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const unsigned long long mine = keys[i];
+    if (mine == 0) continue;
+    int r = 0;
+    for (int j = 0; j < n; ++j) r += keys[j] > mine;
+    if (r < k) out[r] = mine;
+  }
+}
+
+// The block's k best values.  Every thread has the maximum of its values; the
+// k-th largest of 64 group maxima is a threshold that at least k values reach
+// and few exceed.  Only the values of the threads whose maximum reaches it are
+// read again (from L2), the ones above the threshold collected and ranked.
+// Values equal to it are taken in index order: collected too or, where a row
+// has very many (a mask), found by a scan from the front.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* __restrict__ tok,
-                   int V, float c, float inv_t, long long ignore_index, int k,
-                   float* __restrict__ logp,
-                   float* __restrict__ entropy, float* __restrict__ top_logp,
-                   long long* __restrict__ top_tok, float* __restrict__ stats) {
-  ::msb::pdl_begin();
-  __shared__ Sums part[32];
-  __shared__ unsigned long long best[32];
-  const long long r = blockIdx.x;
-  const T* row = logits + r * ld;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-  const long long t = tok[r];
-  if (t == ignore_index) {
-    if (threadIdx.x == 0) {
-      logp[r] = 0.f;
-      if (entropy != nullptr) entropy[r] = 0.f;
+__device__ void top_of_part(const Part<T>& p, float my_max, int k, Shared& sh) {
+  constexpr int N = Vec<T>::N;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  sh.thread_max[tid] = my_max;
+  if (tid < k) sh.best[tid] = 0;
+  if (tid == 0) sh.winners = sh.above = sh.at = 0;
+  __syncthreads();
+  float gmax = -INFINITY;
+  if (tid < kGroups) {
+#pragma unroll
+    for (int j = 0; j < kThreads / kGroups; ++j) gmax = fmaxf(gmax, sh.thread_max[tid + kGroups * j]);
+    sh.group[tid] = order_of(gmax);
+  }
+  __syncthreads();
+  if (tid < kGroups) {
+    const unsigned mine = sh.group[tid];
+    int r = 0;
+#pragma unroll 16
+    for (int j = 0; j < kGroups; ++j) {
+      const unsigned o = sh.group[j];
+      r += o > mine || (o == mine && j < tid);
     }
-    for (int j = threadIdx.x; j < k; j += blockDim.x) {
-      top_logp[r * k + j] = 0.f;
-      top_tok[r * k + j] = -1;
+    if (r == k - 1) sh.threshold = gmax;
+  }
+  __syncthreads();
+  const float thr = sh.threshold;
+  if (my_max >= thr) sh.winner[atomicAdd(&sh.winners, 1)] = (unsigned short)tid;
+  __syncthreads();
+  auto take = [&](float v, int i) {
+    if (v > thr) {
+      const int n = atomicAdd(&sh.above, 1);
+      if (n < kCand) sh.cand[n] = key_of(v, i);
+    } else if (v == thr) {
+      const int n = atomicAdd(&sh.at, 1);
+      if (n < kEqual) sh.equal[n] = key_of(v, i);
     }
+  };
+  const int each = (p.v1 - p.v0 + kThreads - 1) / kThreads, items = sh.winners * each;
+  for (int i = tid; i < items; i += kThreads) {
+    const int w = i / each, v = p.v0 + sh.winner[w] + (i - w * each) * kThreads;
+    if (v >= p.v1) continue;
+    Vec<T> x;
+    x.r = p.mid[v];
+    if (!(x.max() >= thr)) continue;
+    float f[N];
+    x.unpack(f);
+#pragma unroll
+    for (int j = 0; j < N; ++j) take(f[j], p.at(v) + j);
+  }
+  for (int i = tid; i < p.loose(); i += kThreads) {
+    const int at = p.loose_at(i);
+    take(to_f32(p.row[at]), at);
+  }
+  __syncthreads();
+  const int above = sh.above, equal = sh.at;
+  if (above <= kCand) {
+    const int need = min(k - above, equal);
+    if (need > 0 && equal <= kEqual) {   // above < k <= kMaxK: there is room
+      for (int i = tid; i < equal; i += kThreads) sh.cand[above + i] = sh.equal[i];
+      __syncthreads();
+      rank_keys(sh.cand, above + equal, sh.best, k);
+      __syncthreads();
+      return;
+    }
+    // the strictly larger ones, then the first `need` equal ones
+    rank_keys(sh.cand, above, sh.best, k);
+    if (need > 0 && warp == 0) {
+      int found = 0;
+      auto put = [&](bool is, int i) {   // lanes hold ascending indexes
+        const unsigned b = __ballot_sync(0xffffffffu, is);
+        const int r = found + __popc(b & ((1u << lane) - 1u));
+        if (is && r < need) sh.best[above + r] = key_of(thr, i);
+        found += __popc(b);
+      };
+      if (p.first) put(lane < p.head && to_f32(p.row[min(lane, p.V - 1)]) == thr, lane);
+      const int e0 = p.at(p.v0), e1 = p.at(p.v1);
+      for (int i = e0; i < e1 && found < need; i += 32) {
+        const bool in = i + lane < e1;
+        put(in && to_f32(p.row[in ? i + lane : e0]) == thr, i + lane);
+      }
+      if (p.last && found < need) {
+        const int i = p.V - p.tail + lane;
+        put(i < p.V && to_f32(p.row[min(i, p.V - 1)]) == thr, i);
+      }
+    }
+    __syncthreads();
     return;
   }
-  Sums a = {-INFINITY, 0.f, 0.f};
-  for (int i = threadIdx.x; i < V; i += blockDim.x) add(a, to_f32(row[i]), c);
-  a = warp_merge(a, c);
-  if (lane == 0) part[warp] = a;
-  __syncthreads();
-  a = part[0];
-  for (int w = 1; w < nw; ++w) a = merge(a, part[w], c);
-  if (a.m == INFINITY) a.s = NAN;
-  const bool empty = a.m == -INFINITY && a.s == 0.f;
-  const float l2 = log2f(a.s);
-  const float H = kLn2 * (l2 - a.t / a.s);
-  if (threadIdx.x == 0) {
-    const bool in = MSB_OK(t >= 0 && t < V, kSiteLogprobToken, t, V);
-    logp[r] = !in ? NAN : empty ? -INFINITY : (to_f32(row[t]) - a.m) * inv_t - kLn2 * l2;
-    if (entropy != nullptr) entropy[r] = empty || H < 0.f ? 0.f : H;
-    stats[r * 3 + 0] = a.m;
-    stats[r * 3 + 1] = a.s;
-    stats[r * 3 + 2] = a.t;
-  }
+  // more values above the threshold than are kept: the best one k times
   unsigned long long last = ~0ull;
   for (int j = 0; j < k; ++j) {
     unsigned long long b = 0;
-    for (int i = threadIdx.x; i < V; i += blockDim.x) {
-      const unsigned long long q = key_of(to_f32(row[i]), i);
+    auto see = [&](int i) {
+      const unsigned long long q = key_of(to_f32(p.row[i]), i);
       if (q < last && q > b) b = q;
+    };
+    for (int i = p.at(p.v0) + tid; i < p.at(p.v1); i += kThreads) see(i);
+    for (int i = tid; i < p.loose(); i += kThreads) see(p.loose_at(i));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const unsigned long long w = __shfl_xor_sync(0xffffffffu, b, o);
+      b = w > b ? w : b;
     }
-    b = warp_max(b);
     __syncthreads();
-    if (lane == 0) best[warp] = b;
+    if (lane == 0) sh.round[warp] = b;
     __syncthreads();
-    b = best[0];
-    for (int w = 1; w < nw; ++w) b = best[w] > b ? best[w] : b;
+    b = sh.round[0];
+    for (int w = 1; w < kThreads / 32; ++w) b = sh.round[w] > b ? sh.round[w] : b;
     last = b;
-    if (threadIdx.x == 0) {
-      const int i = b == 0 ? 0 : key_index(b);
-      top_tok[r * k + j] = i;
-      top_logp[r * k + j] =
-          empty ? -INFINITY : (to_f32(row[i]) - a.m) * inv_t - kLn2 * l2;
+    if (tid == 0) sh.best[j] = b;
+  }
+  __syncthreads();
+}
+
+// A cluster a row (of one block where there are rows enough).
+template <typename T, bool ENT, bool TOP>
+__global__ void __launch_bounds__(kThreads)
+logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* __restrict__ tok,
+                   int V, float c, float inv_t, long long ignore_index, int k,
+                   float* __restrict__ logp, float* __restrict__ entropy,
+                   float* __restrict__ top_logp, long long* __restrict__ top_tok,
+                   float* __restrict__ stats) {
+  ::msb::pdl_begin();
+  __shared__ Shared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const unsigned R = cluster.num_blocks(), q = cluster.block_rank();
+  const long long r = blockIdx.x / R;
+  const T* row = logits + r * ld;
+  const int tid = threadIdx.x;
+  const long long t = tok[r];
+  if (t == ignore_index) {   // in all blocks of the cluster alike
+    if (q == 0 && tid == 0) {
+      logp[r] = 0.f;
+      if (ENT) entropy[r] = 0.f;
     }
+    if (TOP && q == 0 && tid < k) {
+      top_logp[r * k + tid] = 0.f;
+      top_tok[r * k + tid] = -1;
+    }
+    return;
+  }
+  const bool in = t >= 0 && t < V;
+  const float xt = q == 0 && tid == 0 && in ? to_f32(row[t]) : 0.f;
+  const Part<T> p(row, V, q, R);
+
+  Sums a;
+  constexpr int U = 4;   // vectors in flight a thread
+  for (int v = p.v0 + tid; v < p.v1; v += U * kThreads) {
+    Vec<T> x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (v + u * kThreads < p.v1) {
+        x[u].r = p.mid[v + u * kThreads];
+      } else {
+        x[u].clear();
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) add_vec<T, ENT>(a, x[u], c);
+  }
+  if (tid < p.loose()) add_one<ENT>(a, to_f32(row[p.loose_at(tid)]), c);
+  const float my_max = a.m;
+
+  auto larger = [](float x, float y) { return fmaxf(x, y); };
+  auto sum = [](float x, float y) { return x + y; };
+  float m = block_reduce(my_max, sh.buf[0], larger);
+  if (R > 1) {   // the row's maximum
+    if (tid == 0) sh.ms[0] = m;
+    cluster.sync();
+    for (unsigned b = 0; b < R; ++b) m = fmaxf(m, cluster.map_shared_rank(sh.ms, b)[0]);
+  }
+  const bool wide = is_wide(m, c);
+  float ref = reference(m, c);
+  if (wide && m != INFINITY) {   // once more, with differences
+    a.s = a.t = 0.f;
+    for (int i = p.at(p.v0) + tid; i < p.at(p.v1); i += kThreads)
+      add_z<ENT>((to_f32(row[i]) - m) * c, a.s, a.t);
+    for (int i = tid; i < p.loose(); i += kThreads)
+      add_z<ENT>((to_f32(row[p.loose_at(i)]) - m) * c, a.s, a.t);
+  } else {
+    a.rebase(ref);
+  }
+  float s = block_reduce(a.s, sh.buf[1], sum);
+  float tt = ENT ? block_reduce(a.t, sh.buf[2], sum) : 0.f;
+  if (TOP) top_of_part(p, my_max, k, sh);
+  if (R > 1) {
+    if (tid == 0) {
+      sh.ms[1] = s;
+      sh.ms[2] = tt;
+    }
+    cluster.sync();
+    if (q == 0) {
+      s = tt = 0.f;
+      for (unsigned b = 0; b < R; ++b) {
+        const float* o = cluster.map_shared_rank(sh.ms, b);
+        s += o[1];
+        tt += o[2];
+      }
+      if (TOP) {
+        for (int i = tid; i < (int)R * k; i += kThreads)
+          sh.cand[i] = cluster.map_shared_rank(sh.best, i / k)[i % k];
+      }
+    }
+    cluster.sync();   // the other blocks' shared memory has been read
+    if (q != 0) return;
+    if (TOP) {
+      if (tid < k) sh.best[tid] = 0;
+      __syncthreads();
+      rank_keys(sh.cand, (int)R * k, sh.best, k);
+      __syncthreads();
+    }
+  }
+  if (m == INFINITY) s = NAN;
+  const bool empty = m == -INFINITY && s == 0.f;
+  const float l2 = log2f(s);
+  auto value = [&](float x) {
+    if (empty) return -INFINITY;
+    const float z = fmaf(x, c, -ref);
+    // far below the maximum, z may overflow where the difference does not
+    return wide || z < -1e30f ? (x - m) * inv_t - kLn2 * l2 : kLn2 * (z - l2);
+  };
+  if (tid == 0) {
+    (void)MSB_OK(in, kSiteLogprobToken, t, V);
+    logp[r] = in ? value(xt) : NAN;
+    if (ENT) {
+      const float H = kLn2 * (l2 - tt / s);
+      entropy[r] = empty || H < 0.f ? 0.f : H;
+    }
+    stats[r * 3 + 0] = m;
+    stats[r * 3 + 1] = s;
+    stats[r * 3 + 2] = tt;
+  }
+  if (TOP && tid < k) {
+    const unsigned long long b = sh.best[tid];   // 0: a row of NaN
+    const int i = b == 0 ? 0 : key_index(b);
+    top_tok[r * k + tid] = i;
+    top_logp[r * k + tid] = value(to_f32(row[i]));
   }
 }
 
-// One block a row.  p_i = 2^z_i / s, so with A = -G - gH H and B = -gH,
+// Blocks of a row (splits of them) write dx over its vectors.  p_i = 2^z_i / s,
+// so with A = -G - gH H and B = -gH,
 //   dx_i = p_i (A + B log p_i) / T = 2^z_i (a + b z_i)
 // for b = B ln 2 / (s T) and a = (A - B ln 2 log2 s) / (s T); the entries of
-// the token and the alternatives are written again afterwards.
-template <typename T>
+// the token and the alternatives are written again afterwards.  Rows go from
+// the last to the first: the end of the logits is what the forward left in L2.
+template <typename T, bool ENT>
 __global__ void __launch_bounds__(kThreads)
 logprob_bwd_kernel(const T* __restrict__ logits, long long ld, const long long* __restrict__ tok,
-                   int V, float c, float inv_t, long long ignore_index, int k,
+                   long long M, int V, float c, float inv_t, long long ignore_index, int k,
                    const long long* __restrict__ top_tok, const float* __restrict__ stats,
                    const float* __restrict__ g_logp, const float* __restrict__ g_ent,
-                   const float* __restrict__ g_top, T* __restrict__ dx, long long ld_dx) {
+                   const float* __restrict__ g_top, T* __restrict__ dx, long long ld_dx,
+                   unsigned splits) {
   ::msb::pdl_begin();
-  __shared__ long long at[33];
-  __shared__ float gr[33];
-  const long long r = blockIdx.x;
+  constexpr int N = Vec<T>::N;
+  __shared__ long long at[kMaxK + 1];
+  __shared__ float gr[kMaxK + 1];
+  const long long r = M - 1 - blockIdx.x / splits;
   const T* row = logits + r * ld;
   T* drow = dx + r * ld_dx;
+  const int tid = threadIdx.x;
+  const Part<T> p(row, V, blockIdx.x % splits, splits);
+  const int lo = p.first ? 0 : p.at(p.v0), hi = p.last ? V : p.at(p.v1);
+  // vectors where the two rows are aligned alike
+  const bool vec = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(drow)) & 15) == 0;
+  uint4* dmid = reinterpret_cast<uint4*>(drow + p.head);
   const long long t = tok[r];
-  const float m = stats[r * 3], s = stats[r * 3 + 1], tt = stats[r * 3 + 2];
-  if (t == ignore_index || (m == -INFINITY && s == 0.f)) {
-    for (int i = threadIdx.x; i < V; i += blockDim.x) drow[i] = from_f32<T>(0.f);
+  const bool ignored = t == ignore_index;
+  const float m = ignored ? -INFINITY : stats[r * 3], s = ignored ? 0.f : stats[r * 3 + 1];
+  if (m == -INFINITY && s == 0.f) {
+    const T zero = from_f32<T>(0.f);
+    if (vec) {
+      for (int v = p.v0 + tid; v < p.v1; v += kThreads) dmid[v] = make_uint4(0, 0, 0, 0);
+      if (tid < p.loose()) drow[p.loose_at(tid)] = zero;
+    } else {
+      for (int i = lo + tid; i < hi; i += kThreads) drow[i] = zero;
+    }
     return;
   }
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
     const bool in = t >= 0 && t < V && g_logp != nullptr;
     at[0] = in ? t : -1;
     gr[0] = in ? g_logp[r] : 0.f;
-  } else if (threadIdx.x <= k) {
-    at[threadIdx.x] = g_top != nullptr ? top_tok[r * k + threadIdx.x - 1] : -1;
-    gr[threadIdx.x] = g_top != nullptr ? g_top[r * k + threadIdx.x - 1] : 0.f;
+  } else if (tid <= k) {
+    at[tid] = top_tok[r * k + tid - 1];
+    gr[tid] = g_top[r * k + tid - 1];
   }
   __syncthreads();
   float G = 0.f;
   for (int j = 0; j <= k; ++j) G += gr[j];
-  const float gh = g_ent != nullptr ? g_ent[r] : 0.f;
-  const float l2 = log2f(s), H = kLn2 * (l2 - tt / s), w = inv_t / s;
-  const float b = -gh * kLn2 * w, a = (-G - gh * H) * w - b * l2;
-  auto value = [&](int i) {
-    const float z = fmaxf((to_f32(row[i]) - m) * c, -1e30f);
-    return ex2_approx(z) * (a + b * z);
+  const float l2 = log2f(s), w = inv_t / s;
+  float a = -G * w, b = 0.f;
+  if (ENT) {
+    const float gh = g_ent[r], H = kLn2 * (l2 - stats[r * 3 + 2] / s);
+    b = -gh * kLn2 * w;
+    a = (-G - gh * H) * w - b * l2;
+  }
+  const bool wide = is_wide(m, c);
+  const float ref = reference(m, c);
+  auto of_z = [&](float z) {
+    if (ENT) z = max_nan(z, kLowZ);
+    return ex2_approx(z) * (ENT ? fmaf(b, z, a) : a);
   };
-  for (int i = threadIdx.x; i < V; i += blockDim.x) {
-    const float v = to_f32(row[i]);
-    drow[i] = from_f32<T>(v != v ? NAN : value(i));
+  auto value = [&](float x) { return of_z(wide ? (x - m) * c : fmaf(x, c, -ref)); };
+  if (vec && !wide) {
+    constexpr int U = 4;
+    for (int v = p.v0 + tid; v < p.v1; v += U * kThreads) {
+      Vec<T> x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (v + u * kThreads < p.v1) x[u].r = p.mid[v + u * kThreads];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float f[N];
+        x[u].unpack(f);
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = of_z(fmaf(f[j], c, -ref));
+        uint4 o;
+        if constexpr (N == 8) {
+          o = pack_u4<T>(f);
+        } else {
+          o = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                         __float_as_uint(f[3]));
+        }
+        if (v + u * kThreads < p.v1) dmid[v + u * kThreads] = o;
+      }
+    }
+    if (tid < p.loose()) {
+      const int i = p.loose_at(tid);
+      drow[i] = from_f32<T>(value(to_f32(row[i])));
+    }
+  } else {
+    for (int i = lo + tid; i < hi; i += kThreads) drow[i] = from_f32<T>(value(to_f32(row[i])));
   }
   __syncthreads();
-  if (threadIdx.x <= k && at[threadIdx.x] >= 0) {
+  if (tid <= k && at[tid] >= lo && at[tid] < hi) {
     float g = 0.f;
     bool first = true;
     for (int j = 0; j <= k; ++j) {
-      if (at[j] != at[threadIdx.x]) continue;
-      first = first && j >= (int)threadIdx.x;
+      if (at[j] != at[tid]) continue;
+      first = first && j >= tid;
       g += gr[j];
     }
     if (first) {
-      const int i = (int)at[threadIdx.x];
-      drow[i] = from_f32<T>(value(i) + g * inv_t);
+      const int i = (int)at[tid];
+      drow[i] = from_f32<T>(value(to_f32(row[i])) + g * inv_t);
     }
   }
+}
+
+// Blocks a row: twice the SMs' number in all where rows are few, as long as a
+// block keeps half of its threads busy with a vector.
+unsigned blocks_a_row(long long M, int V, int per_vec) {
+  unsigned R = 1;
+  while (R < kMaxCluster && M * R < 2 * kNumSMs && V / (int)(2 * R) >= per_vec * kThreads / 2) R *= 2;
+  return R;
 }
 
 }  // namespace
@@ -221,9 +598,18 @@ void logprob_fwd(const void* logits, long long ld, const long long* tok, long lo
                  float* top_logp, long long* top_tok, float* stats, int dtype, cudaStream_t st) {
   if (M == 0) return;
   const float c = (float)(1.4426950408889634 / (double)temperature);
+  const float inv_t = (float)(1.0 / (double)temperature);
   MSB_DISPATCH_FLOAT(dtype, T, {
-    launch(logprob_fwd_kernel<T>, (unsigned)M, kThreads, 0, st, (const T*)logits, ld, tok, V, c,
-           (float)(1.0 / temperature), ignore_index, k, logp, entropy, top_logp, top_tok, stats);
+    const unsigned R = blocks_a_row(M, V, Vec<T>::N);
+    auto go = [&](auto* kernel) {
+      launch_cluster(R, kernel, (unsigned)M * R, kThreads, 0, st, (const T*)logits, ld, tok, V, c,
+                     inv_t, ignore_index, k, logp, entropy, top_logp, top_tok, stats);
+    };
+    if (entropy != nullptr) {
+      k > 0 ? go(logprob_fwd_kernel<T, true, true>) : go(logprob_fwd_kernel<T, true, false>);
+    } else {
+      k > 0 ? go(logprob_fwd_kernel<T, false, true>) : go(logprob_fwd_kernel<T, false, false>);
+    }
   });
   MSB_CHECK_LAUNCH("logprob_fwd");
 }
@@ -233,11 +619,15 @@ void logprob_bwd(const void* logits, long long ld, const long long* tok, long lo
                  const float* stats, const float* g_logp, const float* g_ent, const float* g_top,
                  void* dx, long long ld_dx, int dtype, cudaStream_t st) {
   if (M == 0) return;
-  const double c = 1.4426950408889634 / (double)temperature;
+  const float c = (float)(1.4426950408889634 / (double)temperature);
+  const float inv_t = (float)(1.0 / (double)temperature);
   MSB_DISPATCH_FLOAT(dtype, T, {
-    launch(logprob_bwd_kernel<T>, (unsigned)M, kThreads, 0, st, (const T*)logits, ld, tok, V,
-           (float)c, (float)(1.0 / temperature), ignore_index, k, top_tok, stats, g_logp, g_ent,
-           g_top, (T*)dx, ld_dx);
+    const unsigned R = blocks_a_row(M, V, Vec<T>::N);
+    auto go = [&](auto* kernel) {
+      launch(kernel, (unsigned)M * R, kThreads, 0, st, (const T*)logits, ld, tok, M, V, c, inv_t,
+             ignore_index, k, top_tok, stats, g_logp, g_ent, g_top, (T*)dx, ld_dx, R);
+    };
+    g_ent != nullptr ? go(logprob_bwd_kernel<T, true>) : go(logprob_bwd_kernel<T, false>);
   });
   MSB_CHECK_LAUNCH("logprob_bwd");
 }

@@ -707,7 +707,8 @@ def _token_logprobs_torch(logits, tokens, temperature, entropy, top_k, ignore_in
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 1.0,
                    entropy: bool = False, top_k: int = 0, ignore_index: int = -100
                    ) -> TokenLogprobs:
-    """Log probabilities of ``tokens`` under softmax(``logits`` / ``temperature``).
+    """Log probabilities of ``tokens`` under softmax(``logits`` / ``temperature``),
+    for a temperature between 1e-30 and 1e30.
 
     ``logits`` [..., V] in fp32, fp16 or bf16 (rows may be padded, as
     ``linear(pad_out=)`` leaves them) and int64 ``tokens`` [...].  All results
@@ -741,8 +742,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     if not 0 <= top_k <= min(MAX_TOP_K, V):
         raise ValueError(f"token_logprobs: top_k must be between 0 and {min(MAX_TOP_K, V)}, "
                          f"got {top_k}")
-    if not (math.isfinite(temperature) and temperature > 0):
-        raise ValueError(f"token_logprobs: temperature must be positive, got {temperature}")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"token_logprobs: temperature must be between 1e-30 and 1e30, got "
+                         f"{temperature}")
     args = (float(temperature), bool(entropy), int(top_k), int(ignore_index))
     if logits.is_cuda and logits.numel():
         return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, *args))
