@@ -78,42 +78,63 @@ __device__ __forceinline__ unsigned amax8(const float (&f)[8]) {
   return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
 }
 
-// D % 8 == 0 and 16-byte aligned rows: four lanes a block, eight values each.
+// The vector kernels: widths that are a multiple of 8 and 16-byte aligned rows,
+// four lanes a block, eight values a lane.  A thread has two vectors in flight,
+// a grid's width apart.  The number of vectors of a launch fits 31 bits.
+constexpr int kThreads = 256;
+constexpr int kFlight = 2;
+
 template <typename T>
-__global__ void __launch_bounds__(256)
-pack8_vec_kernel(const T* __restrict__ x, long long ld, long long total, int D, int nb,
+__global__ void __launch_bounds__(kThreads)
+pack8_vec_kernel(const T* __restrict__ x, long long ld, unsigned total, int D, FastDiv nv,
                  uint2* __restrict__ codes, unsigned char* __restrict__ scales) {
   ::msb::pdl_begin();
-  const unsigned lane = threadIdx.x & 31;
-  const int nv = nb * 4;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i - lane < total;
-       i += (long long)gridDim.x * blockDim.x) {
-    const long long row = i / nv;
-    const int c = (int)(i - row * nv) * 8;
-    float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (i < total && c < D) load8(x + row * ld + c, f);
-    const unsigned b = scale_byte(amax8(f));
-    if (i < total) {
-      codes[i] = codes8(f, code_mul(b));
-      if ((lane & 3) == 0) scales[i >> 2] = (unsigned char)b;
+  const unsigned lane = threadIdx.x & 31, step = gridDim.x * kThreads;
+  for (unsigned i0 = blockIdx.x * kThreads + threadIdx.x; i0 - lane < total; i0 += kFlight * step) {
+    float f[kFlight][8];
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      const unsigned i = i0 + u * step, row = nv.div(i), c = (i - row * nv.d) * 8;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[u][k] = 0.f;
+      if (i < total && c < D) load8(x + row * ld + c, f[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      const unsigned i = i0 + u * step;
+      const unsigned b = scale_byte(amax8(f[u]));
+      if (i < total) {
+        codes[i] = codes8(f[u], code_mul(b));
+        if ((lane & 3) == 0) scales[i >> 2] = (unsigned char)b;
+      }
     }
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kThreads)
 unpack8_vec_kernel(const uint2* __restrict__ codes, const unsigned char* __restrict__ scales,
-                   T* __restrict__ x, long long total, int D, int nb) {
+                   T* __restrict__ x, unsigned total, int D, FastDiv nv) {
   ::msb::pdl_begin();
-  const int nv = nb * 4;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (long long)gridDim.x * blockDim.x) {
-    const long long row = i / nv;
-    const int c = (int)(i - row * nv) * 8;
-    if (c >= D) continue;
-    float f[8];
-    values8(codes[i], code_scale(scales[i >> 2]), f);
-    store8(x + row * D + c, f);
+  const unsigned step = gridDim.x * kThreads;
+  for (unsigned i0 = blockIdx.x * kThreads + threadIdx.x; i0 < total; i0 += kFlight * step) {
+    uint2 w[kFlight];
+    unsigned b[kFlight];
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      const unsigned i = i0 + u * step;
+      if (i >= total) continue;
+      w[u] = codes[i];
+      b[u] = scales[i >> 2];
+    }
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      const unsigned i = i0 + u * step, row = nv.div(i), c = (i - row * nv.d) * 8;
+      if (i >= total || c >= D) continue;
+      float f[8];
+      values8(w[u], code_scale(b[u]), f);
+      store8(x + (long long)row * D + c, f);
+    }
   }
 }
 
@@ -151,10 +172,12 @@ unpack8_any_kernel(const signed char* __restrict__ codes, const unsigned char* _
   }
 }
 
-__device__ __forceinline__ float silu_f(float g) { return g / (1.f + __expf(-g)); }
+// quotients by __fdividef: 2 units in the last place, and 0 where 1 + e^-g
+// passes 2^126, as the rounded quotient nearly is
+__device__ __forceinline__ float silu_f(float g) { return __fdividef(g, 1.f + __expf(-g)); }
 // h = silu(g) u:  dg = dh u s (1 + g (1 - s)),  du = dh g s,  s = sigmoid(g)
 __device__ __forceinline__ void swiglu_grad(float dh, float g, float u, float& dg, float& du) {
-  const float s = 1.f / (1.f + __expf(-g));
+  const float s = __fdividef(1.f, 1.f + __expf(-g));
   dg = dh * u * s * (1.f + g * (1.f - s));
   du = dh * g * s;
 }
@@ -163,61 +186,79 @@ __device__ __forceinline__ void swiglu_grad(float dh, float g, float u, float& d
 // 2r + 1 of width F, so each has blocks of its own.  Without codes (nullptr)
 // only h is written.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kThreads)
 swiglu8_fwd_vec_kernel(const T* __restrict__ gu, T* __restrict__ h, uint2* __restrict__ codes,
-                       unsigned char* __restrict__ scales, long long total, int F, int nb) {
+                       unsigned char* __restrict__ scales, unsigned total, int F, FastDiv nv) {
   ::msb::pdl_begin();
-  const unsigned lane = threadIdx.x & 31;
-  const int nv = nb * 4;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i - lane < total;
-       i += (long long)gridDim.x * blockDim.x) {
-    const long long row = i / nv;
-    const int v = (int)(i - row * nv), c = v * 8;
-    const bool in = i < total && c < F;
-    float g[8] = {0, 0, 0, 0, 0, 0, 0, 0}, u[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (in) {
-      load8(gu + row * 2 * F + c, g);
-      load8(gu + row * 2 * F + F + c, u);
-    }
-    const unsigned bg = scale_byte(amax8(g)), bu = scale_byte(amax8(u));
-    if (codes != nullptr && i < total) {
-      const long long at = row * 2 * nv + v;
-      codes[at] = codes8(g, code_mul(bg));
-      codes[at + nv] = codes8(u, code_mul(bu));
-      if ((lane & 3) == 0) {
-        scales[at >> 2] = (unsigned char)bg;
-        scales[(at + nv) >> 2] = (unsigned char)bu;
+  const unsigned lane = threadIdx.x & 31, step = gridDim.x * kThreads;
+  for (unsigned i0 = blockIdx.x * kThreads + threadIdx.x; i0 - lane < total; i0 += kFlight * step) {
+    float g[kFlight][8], u[kFlight][8];
+#pragma unroll
+    for (int j = 0; j < kFlight; ++j) {
+      const unsigned i = i0 + j * step, row = nv.div(i), c = (i - row * nv.d) * 8;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g[j][k] = u[j][k] = 0.f;
+      if (i < total && c < F) {
+        load8(gu + (long long)row * 2 * F + c, g[j]);
+        load8(gu + (long long)row * 2 * F + F + c, u[j]);
       }
     }
-    if (in) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) g[k] = silu_f(g[k]) * u[k];
-      store8(h + row * F + c, g);
+    for (int j = 0; j < kFlight; ++j) {
+      const unsigned i = i0 + j * step, row = nv.div(i), v = i - row * nv.d, c = v * 8;
+      const unsigned bg = scale_byte(amax8(g[j])), bu = scale_byte(amax8(u[j]));
+      if (codes != nullptr && i < total) {
+        const long long at = (long long)row * 2 * nv.d + v;
+        codes[at] = codes8(g[j], code_mul(bg));
+        codes[at + nv.d] = codes8(u[j], code_mul(bu));
+        if ((lane & 3) == 0) {
+          scales[at >> 2] = (unsigned char)bg;
+          scales[(at + nv.d) >> 2] = (unsigned char)bu;
+        }
+      }
+      if (i < total && c < F) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) g[j][k] = silu_f(g[j][k]) * u[j][k];
+        store8(h + (long long)row * F + c, g[j]);
+      }
     }
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kThreads)
 swiglu8_bwd_vec_kernel(const T* __restrict__ dh, const uint2* __restrict__ codes,
                        const unsigned char* __restrict__ scales, T* __restrict__ dgu,
-                       long long total, int F, int nb) {
+                       unsigned total, int F, FastDiv nv) {
   ::msb::pdl_begin();
-  const int nv = nb * 4;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (long long)gridDim.x * blockDim.x) {
-    const long long row = i / nv;
-    const int v = (int)(i - row * nv), c = v * 8;
-    if (c >= F) continue;
-    const long long at = row * 2 * nv + v;
-    float d[8], g[8], u[8];
-    load8(dh + row * F + c, d);
-    values8(codes[at], code_scale(scales[at >> 2]), g);
-    values8(codes[at + nv], code_scale(scales[(at + nv) >> 2]), u);
+  const unsigned step = gridDim.x * kThreads;
+  for (unsigned i0 = blockIdx.x * kThreads + threadIdx.x; i0 < total; i0 += kFlight * step) {
+    float d[kFlight][8];
+    uint2 wg[kFlight], wu[kFlight];
+    unsigned bg[kFlight], bu[kFlight];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) swiglu_grad(d[k], g[k], u[k], g[k], u[k]);
-    store8(dgu + row * 2 * F + c, g);
-    store8(dgu + row * 2 * F + F + c, u);
+    for (int j = 0; j < kFlight; ++j) {
+      const unsigned i = i0 + j * step, row = nv.div(i), v = i - row * nv.d, c = v * 8;
+      if (i >= total || c >= F) continue;
+      const long long at = (long long)row * 2 * nv.d + v;
+      wg[j] = codes[at];
+      wu[j] = codes[at + nv.d];
+      bg[j] = scales[at >> 2];
+      bu[j] = scales[(at + nv.d) >> 2];
+      load8(dh + (long long)row * F + c, d[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kFlight; ++j) {
+      const unsigned i = i0 + j * step, row = nv.div(i), c = (i - row * nv.d) * 8;
+      if (i >= total || c >= F) continue;
+      float g[8], u[8];
+      values8(wg[j], code_scale(bg[j]), g);
+      values8(wu[j], code_scale(bu[j]), u);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) swiglu_grad(d[j][k], g[k], u[k], g[k], u[k]);
+      store8(dgu + (long long)row * 2 * F + c, g);
+      store8(dgu + (long long)row * 2 * F + F + c, u);
+    }
   }
 }
 
@@ -275,23 +316,32 @@ swiglu8_bwd_any_kernel(const T* __restrict__ dh, const signed char* __restrict__
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// a grid that fills the GPU with 256-thread blocks, eight a SM, and loops
-int loop_grid(long long threads) { return grid_for(threads, 256, kNumSMs * 8); }
+// a grid of 256-thread blocks that fills the GPU, eight a SM, and loops
+int loop_grid(long long threads) { return grid_for(threads, kThreads, kNumSMs * 8); }
+
+// f(first row, rows) over parts of at most 2^30 vectors, nv a row
+template <typename F>
+void in_parts(long long rows, int nv, F&& f) {
+  const long long most = (1LL << 30) / nv > 0 ? (1LL << 30) / nv : 1;
+  for (long long r = 0; r < rows; r += most) f(r, rows - r < most ? rows - r : most);
+}
 
 }  // namespace
 
 void pack8(const void* x, long long ld, signed char* codes, unsigned char* scales, long long rows,
            int D, int dtype, cudaStream_t st) {
   const int nb = (D + kBlk - 1) / kBlk;
-  if (rows == 0) return;
   MSB_DISPATCH_FLOAT(dtype, T, {
+    const T* in = (const T*)x;
     if (D % 8 == 0 && aligned16(x) && (ld * sizeof(T)) % 16 == 0) {
-      const long long total = rows * nb * 4;
-      launch(pack8_vec_kernel<T>, loop_grid(total), 256, 0, st, (const T*)x, ld, total, D, nb,
-             (uint2*)codes, scales);
-    } else {
-      launch(pack8_any_kernel<T>, loop_grid(rows * nb * 32), 256, 0, st, (const T*)x, ld,
-             rows * nb, D, nb, codes, scales);
+      in_parts(rows, nb * 4, [&](long long r, long long n) {
+        launch(pack8_vec_kernel<T>, loop_grid(n * nb * 4 / kFlight), kThreads, 0, st, in + r * ld,
+               ld, (unsigned)(n * nb * 4), D, FastDiv(nb * 4), (uint2*)(codes + r * nb * kBlk),
+               scales + r * nb);
+      });
+    } else if (rows > 0) {
+      launch(pack8_any_kernel<T>, loop_grid(rows * nb * 32), kThreads, 0, st, in, ld, rows * nb, D,
+             nb, codes, scales);
     }
   });
   MSB_CHECK_LAUNCH("pack8");
@@ -300,15 +350,16 @@ void pack8(const void* x, long long ld, signed char* codes, unsigned char* scale
 void unpack8(const signed char* codes, const unsigned char* scales, void* x, long long rows, int D,
              int dtype, cudaStream_t st) {
   const int nb = (D + kBlk - 1) / kBlk;
-  if (rows == 0) return;
   MSB_DISPATCH_FLOAT(dtype, T, {
-    if ((D * sizeof(T)) % 16 == 0 && D % 8 == 0) {
-      const long long total = rows * nb * 4;
-      launch(unpack8_vec_kernel<T>, loop_grid(total), 256, 0, st, (const uint2*)codes, scales,
-             (T*)x, total, D, nb);
-    } else {
-      launch(unpack8_any_kernel<T>, loop_grid(rows * nb * 32), 256, 0, st, codes, scales, (T*)x,
-             rows * nb, D, nb);
+    if (D % 8 == 0) {
+      in_parts(rows, nb * 4, [&](long long r, long long n) {
+        launch(unpack8_vec_kernel<T>, loop_grid(n * nb * 4 / kFlight), kThreads, 0, st,
+               (const uint2*)(codes + r * nb * kBlk), scales + r * nb, (T*)x + r * D,
+               (unsigned)(n * nb * 4), D, FastDiv(nb * 4));
+      });
+    } else if (rows > 0) {
+      launch(unpack8_any_kernel<T>, loop_grid(rows * nb * 32), kThreads, 0, st, codes, scales,
+             (T*)x, rows * nb, D, nb);
     }
   });
   MSB_CHECK_LAUNCH("unpack8");
@@ -317,14 +368,16 @@ void unpack8(const signed char* codes, const unsigned char* scales, void* x, lon
 void swiglu8_fwd(const void* gu, void* h, signed char* codes, unsigned char* scales,
                  long long rows, int F, int dtype, cudaStream_t st) {
   const int nb = (F + kBlk - 1) / kBlk;
-  if (rows == 0) return;
   MSB_DISPATCH_FLOAT(dtype, T, {
     if (F % 8 == 0 && aligned16(gu)) {
-      const long long total = rows * nb * 4;
-      launch(swiglu8_fwd_vec_kernel<T>, loop_grid(total), 256, 0, st, (const T*)gu, (T*)h,
-             (uint2*)codes, scales, total, F, nb);
-    } else {
-      launch(swiglu8_fwd_any_kernel<T>, loop_grid(rows * nb * 32), 256, 0, st, (const T*)gu,
+      in_parts(rows, nb * 4, [&](long long r, long long n) {
+        launch(swiglu8_fwd_vec_kernel<T>, loop_grid(n * nb * 4 / kFlight), kThreads, 0, st,
+               (const T*)gu + r * 2 * F, (T*)h + r * F,
+               codes == nullptr ? nullptr : (uint2*)(codes + r * 2 * nb * kBlk),
+               scales + r * 2 * nb, (unsigned)(n * nb * 4), F, FastDiv(nb * 4));
+      });
+    } else if (rows > 0) {
+      launch(swiglu8_fwd_any_kernel<T>, loop_grid(rows * nb * 32), kThreads, 0, st, (const T*)gu,
              (T*)h, codes, scales, rows * nb, F, nb);
     }
   });
@@ -334,14 +387,16 @@ void swiglu8_fwd(const void* gu, void* h, signed char* codes, unsigned char* sca
 void swiglu8_bwd(const void* dh, const signed char* codes, const unsigned char* scales, void* dgu,
                  long long rows, int F, int dtype, cudaStream_t st) {
   const int nb = (F + kBlk - 1) / kBlk;
-  if (rows == 0) return;
   MSB_DISPATCH_FLOAT(dtype, T, {
     if (F % 8 == 0 && aligned16(dh)) {
-      const long long total = rows * nb * 4;
-      launch(swiglu8_bwd_vec_kernel<T>, loop_grid(total), 256, 0, st, (const T*)dh,
-             (const uint2*)codes, scales, (T*)dgu, total, F, nb);
-    } else {
-      launch(swiglu8_bwd_any_kernel<T>, loop_grid(rows * nb * 32), 256, 0, st, (const T*)dh,
+      in_parts(rows, nb * 4, [&](long long r, long long n) {
+        launch(swiglu8_bwd_vec_kernel<T>, loop_grid(n * nb * 4 / kFlight), kThreads, 0, st,
+               (const T*)dh + r * F, (const uint2*)(codes + r * 2 * nb * kBlk),
+               scales + r * 2 * nb, (T*)dgu + r * 2 * F, (unsigned)(n * nb * 4), F,
+               FastDiv(nb * 4));
+      });
+    } else if (rows > 0) {
+      launch(swiglu8_bwd_any_kernel<T>, loop_grid(rows * nb * 32), kThreads, 0, st, (const T*)dh,
              codes, scales, (T*)dgu, rows * nb, F, nb);
     }
   });

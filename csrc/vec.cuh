@@ -86,5 +86,20 @@ __device__ __forceinline__ uint4 pack_u4(const float (&f)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// n / d for 0 <= n < 2^31 by a multiplication: m = ceil(2^p / d) with
+// p = 31 + ceil(log2 d) gives floor(n m / 2^p) = floor(n / d) there (Granlund
+// and Montgomery 1994).  A 64-bit division costs more than the rest of a
+// streaming kernel's loop.
+struct FastDiv {
+  unsigned d, m, s;
+  explicit FastDiv(unsigned d_) : d(d_), m(0), s(0) {
+    while ((1u << s) < d) ++s;
+    if (s > 0) m = (unsigned)(((1ull << (31 + s)) + d - 1) / d);
+  }
+  __device__ __forceinline__ unsigned div(unsigned n) const {
+    return s == 0 ? n : __umulhi(n, m) >> (s - 1);
+  }
+};
+
 }  // namespace
 }  // namespace msb
