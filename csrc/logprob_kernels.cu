@@ -86,12 +86,6 @@ __device__ __forceinline__ int key_index(unsigned long long k) {
   return (int)(0xffffffffu - (unsigned)k);
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
 // The exponents of a row are z = x c - m c, one fused operation on the rounded
 // product m c (the same one wherever the row's z are computed, so its rounding
 // cancels).  Where m c comes near fp32's range (the lowest value of fp32 or bf16

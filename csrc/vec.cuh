@@ -23,6 +23,19 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
+// 1 / x to 1 unit in the last place
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// max that is NaN where either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // 8-element accesses: one 16-byte transaction when the address allows it,
 // element-wise otherwise.  Parameters are views into a flat arena at
 // arbitrary element offsets, so weights and biases need not be aligned.
