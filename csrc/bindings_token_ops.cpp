@@ -219,7 +219,8 @@ at::Tensor scaled_embedding_bwd(const at::Tensor& dout, const at::Tensor& idx, i
   check_contig(dout, "dout");
   const int64_t n = idx.numel(), C = dout.size(-1);
   TORCH_CHECK(dout.dim() >= 1 && C > 0 && dout.numel() == n * C, "dout: [tokens, C]");
-  TORCH_CHECK(V > 0 && V < (1LL << 31) && n < (1LL << 31) && C < (1LL << 30), "too large");
+  TORCH_CHECK(V > 0 && V < (1LL << 31) && n < (1LL << 31) && C < (1LL << 30) &&
+                  n * ((C + 255) / 256) < (1LL << 34), "too large");
   const long long* tok = tokens_of(idx, n, dout);
   c10::cuda::CUDAGuard g(dout.device());
   at::Tensor grad;
@@ -230,7 +231,7 @@ at::Tensor scaled_embedding_bwd(const at::Tensor& dout, const at::Tensor& idx, i
                 "sink: a [V, C] gradient of dout's type");
     grad = *sink;
   } else {
-    grad = at::zeros({V, C}, dout.options());
+    grad = at::empty({V, C}, dout.options());   // cleared beside the sorting
   }
   at::Tensor ws = at::empty({msb::scaled_embedding_ws(n, (int)C)}, dout.options().dtype(at::kInt));
   msb::scaled_embedding_bwd(dout.data_ptr(), tok, grad.data_ptr(), given(sink),

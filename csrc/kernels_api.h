@@ -121,9 +121,9 @@ void logprob_bwd(const void* logits, long long ld, const long long* tok, long lo
                  float temperature, long long ignore_index, int k, const long long* top_tok,
                  const float* stats, const float* g_logp, const float* g_ent, const float* g_top,
                  void* dx, long long ld_dx, int dtype, cudaStream_t st);
-// embedding with scaling (embedding_sorted.cu); the backward writes the rows of
-// the tokens that occur (grad is zero elsewhere already) or adds to them, and
-// needs scaled_embedding_ws words of scratch; padding < 0: none
+// embedding with scaling (embedding_sorted.cu); the backward writes all of grad
+// or, with `accumulate`, adds to the rows of the tokens that occur; it needs
+// scaled_embedding_ws words of scratch; padding < 0: none
 void scaled_embedding_fwd(const long long* idx, const void* w, void* out, long long n, int C,
                           long long V, float scale, int dtype, cudaStream_t st);
 long long scaled_embedding_ws(long long n, int C);
