@@ -14,6 +14,8 @@
 // gradient (key V, sorted behind all others).
 #include <cooperative_groups.h>
 
+#include <utility>
+
 #include "common.cuh"
 #include "vec.cuh"
 
@@ -65,19 +67,19 @@ scaled_embedding_fwd_kernel(const long long* __restrict__ idx, const T* __restri
 //
 // Every warp of the cluster owns one contiguous piece of the list.  A pass
 // counts the digits of each warp's piece, turns the counts into places (over
-// the warps of a block, over the blocks through distributed shared memory, over
-// the digits), and writes each entry to its place, warp by warp in order, lanes
-// with the same digit ranked by __match_any_sync: stable by construction.  The
-// cluster barrier orders the passes.  What bounds it is the latency of its
-// steps, not their work: 16384 tokens of 50257 take SORT16K us.
+// the warps of a block, over the blocks, each of which writes its totals into
+// the others' shared memory, over the digits), and writes each entry to its
+// place, warp by warp in order, lanes with the same digit ranked by ballots on
+// its bits (__match_any_sync took seven times as long): stable by construction.
+// The cluster barrier orders the passes.  What bounds it is the latency of its
+// steps: 16384 tokens of 50257 take SORT16K us.
 __global__ void __launch_bounds__(kSortThreads)
 sort_tokens_kernel(const long long* __restrict__ idx, long long n, long long V,
-                   long long padding, int passes, int bits, unsigned* key_a, unsigned* pos_a,
-                   unsigned* key_b, unsigned* pos_b, uint4* fill, long long fill_n,
-                   int fill_tail) {
+                   long long padding, int passes, int bits, uint2* list_a, uint2* list_b,
+                   unsigned* open_runs, uint4* fill, long long fill_n, int fill_tail) {
   ::msb::pdl_begin();
   extern __shared__ unsigned cnt[];   // [kSortWarps][1 << bits]
-  __shared__ unsigned hist[kBins], base[kBins], wsum[kSortWarps];
+  __shared__ unsigned hist[kMaxCluster][kBins], base[kBins], wsum[kSortWarps], quarter[4][kBins];
   cg::cluster_group cluster = cg::this_cluster();
   const unsigned q = cluster.block_rank(), R = cluster.num_blocks();
   if (blockIdx.x >= R) {
@@ -87,75 +89,90 @@ sort_tokens_kernel(const long long* __restrict__ idx, long long n, long long V,
     if (first < fill_tail) reinterpret_cast<unsigned char*>(fill + fill_n)[first] = 0;
     return;
   }
+  if (passes == 0) return;
+  auto started = cluster.barrier_arrive();   // waited for before another block's memory is written
+  if (blockIdx.x == 0 && threadIdx.x == 0) *open_runs = 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int bins = 1 << bits;
   const unsigned ones = (unsigned)bins - 1u, below = (1u << lane) - 1u;
   const long long per = (n + (long long)R * kSortThreads - 1) / ((long long)R * kSortThreads) * 32;
   const long long lo = min(n, per * (q * kSortWarps + warp)), hi = min(n, lo + per);
   unsigned* mine = cnt + warp * bins;
-  // entry i of a pass; behind the piece: a digit of its own, so that lanes match
-  auto load = [&](int p, long long i, unsigned& key, unsigned& pos) {
-    key = pos = 0;
-    if (i >= hi) return;
-    if (p == 0) {
-      const long long t = idx[i];
-      const bool in = t >= 0 && t < V;
-      key = in && t != padding ? (unsigned)t : (unsigned)V;
-      pos = (unsigned)i;
-    } else {   // written by other blocks of the cluster
-      key = __ldcg((p & 1 ? key_a : key_b) + i);
-      pos = __ldcg((p & 1 ? pos_a : pos_b) + i);
-    }
+  auto load = [&](int p, long long i) {   // (token, position) of entry i
+    if (i >= hi) return make_uint2(0u, 0u);
+    if (p > 0) return __ldcg((p & 1 ? list_a : list_b) + i);   // other blocks wrote it
+    const long long t = idx[i];
+    return make_uint2(t >= 0 && t < V && t != padding ? (unsigned)t : (unsigned)V, (unsigned)i);
   };
   for (int p = 0; p < passes; ++p) {
     const int shift = p * bits;
-    unsigned key[kHeld], pos[kHeld], same[kHeld];
+    uint2 held[kHeld];
+    unsigned same[kHeld];
 #pragma unroll
-    for (int h = 0; h < kHeld; ++h) load(p, lo + h * 32 + lane, key[h], pos[h]);
+    for (int h = 0; h < kHeld; ++h) held[h] = load(p, lo + h * 32 + lane);
     for (int b = lane * 4; b < bins; b += 128)
       *reinterpret_cast<uint4*>(mine + b) = make_uint4(0, 0, 0, 0);
     __syncwarp();
-    auto match = [&](unsigned k, long long i) {
-      return __match_any_sync(0xffffffffu, i < hi ? (k >> shift) & ones : kBins);
+    auto match = [&](unsigned key, long long i) {   // the lanes with this lane's digit
+      const unsigned d = (key >> shift) & ones;
+      unsigned m = __ballot_sync(0xffffffffu, i < hi);
+      for (int b = 0; b < bits; ++b) {
+        const unsigned v = __ballot_sync(0xffffffffu, d >> b & 1);
+        m &= d >> b & 1 ? v : ~v;
+      }
+      return m;
     };
-    auto count = [&](unsigned k, long long i, unsigned m) {
-      if (i < hi && (m & below) == 0) mine[(k >> shift) & ones] += __popc(m);
+    auto count = [&](unsigned key, long long i, unsigned m) {
+      if (i < hi && (m & below) == 0) mine[(key >> shift) & ones] += __popc(m);
       __syncwarp();
     };
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {
       if (lo + h * 32 < hi) {
-        same[h] = match(key[h], lo + h * 32 + lane);
-        count(key[h], lo + h * 32 + lane, same[h]);
+        same[h] = match(held[h].x, lo + h * 32 + lane);
+        count(held[h].x, lo + h * 32 + lane, same[h]);
       }
     }
     for (long long i0 = lo + kHeld * 32; i0 < hi; i0 += 32) {
-      unsigned k, at;
-      load(p, i0 + lane, k, at);
-      count(k, i0 + lane, match(k, i0 + lane));
+      const unsigned key = load(p, i0 + lane).x;
+      count(key, i0 + lane, match(key, i0 + lane));
     }
     __syncthreads();
+    // where each warp's entries of a digit begin among the block's: sums over
+    // the warps, a quarter of them a thread
+    for (int t = threadIdx.x; t < 4 * bins; t += kSortThreads) {
+      const int d = t & (bins - 1), part = t >> bits;
+      unsigned run = 0;
+#pragma unroll
+      for (int w = 0; w < kSortWarps / 4; ++w) {
+        unsigned* at = cnt + (part * (kSortWarps / 4) + w) * bins + d;
+        const unsigned v = *at;
+        *at = run;
+        run += v;
+      }
+      quarter[part][d] = run;
+    }
+    __syncthreads();
+    if (p == 0) cluster.barrier_wait(std::move(started));
     if (threadIdx.x < bins) {
       unsigned run = 0;
 #pragma unroll
-      for (int w = 0; w < kSortWarps; ++w) {
-        const unsigned v = cnt[w * bins + threadIdx.x];
-        cnt[w * bins + threadIdx.x] = run;
+      for (int k = 0; k < 4; ++k) {
+        const unsigned v = quarter[k][threadIdx.x];
+        quarter[k][threadIdx.x] = run;
         run += v;
       }
-      hist[threadIdx.x] = run;
+      for (unsigned r = 0; r < R; ++r)
+        cluster.map_shared_rank(&hist[0][0], r)[q * kBins + threadIdx.x] = run;
     }
     cluster.sync();
     unsigned before = 0, all = 0;
     if (threadIdx.x < bins) {
-      unsigned v[kMaxCluster];
-#pragma unroll
-      for (unsigned r = 0; r < kMaxCluster; ++r)
-        v[r] = r < R ? *cluster.map_shared_rank(hist + threadIdx.x, r) : 0u;
 #pragma unroll
       for (unsigned r = 0; r < kMaxCluster; ++r) {
-        before += r < q ? v[r] : 0u;
-        all += v[r];
+        const unsigned v = r < R ? hist[r][threadIdx.x] : 0u;
+        before += r < q ? v : 0u;
+        all += v;
       }
     }
     unsigned incl = all;
@@ -169,27 +186,22 @@ sort_tokens_kernel(const long long* __restrict__ idx, long long n, long long V,
     const unsigned lower = __reduce_add_sync(0xffffffffu, lane < warp ? wsum[lane] : 0u);
     if (threadIdx.x < bins) base[threadIdx.x] = lower + incl - all + before;
     __syncthreads();
-    unsigned* key_out = p & 1 ? key_b : key_a;
-    unsigned* pos_out = p & 1 ? pos_b : pos_a;
-    auto place = [&](unsigned k, unsigned from, long long i, unsigned m) {
-      const unsigned d = (k >> shift) & ones;
-      if (i < hi) {
-        const unsigned at = base[d] + mine[d] + __popc(m & below);
-        key_out[at] = k;
-        pos_out[at] = from;
-      }
+    uint2* out = p & 1 ? list_b : list_a;
+    const unsigned* ahead = quarter[warp / (kSortWarps / 4)];
+    auto place = [&](uint2 e, long long i, unsigned m) {
+      const unsigned d = (e.x >> shift) & ones;
+      if (i < hi) out[base[d] + ahead[d] + mine[d] + __popc(m & below)] = e;
       __syncwarp();
       if (i < hi && (m & below) == 0) mine[d] += __popc(m);
       __syncwarp();
     };
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {
-      if (lo + h * 32 < hi) place(key[h], pos[h], lo + h * 32 + lane, same[h]);
+      if (lo + h * 32 < hi) place(held[h], lo + h * 32 + lane, same[h]);
     }
     for (long long i0 = lo + kHeld * 32; i0 < hi; i0 += 32) {
-      unsigned k, from;
-      load(p, i0 + lane, k, from);
-      place(k, from, i0 + lane, match(k, i0 + lane));
+      const uint2 e = load(p, i0 + lane);
+      place(e, i0 + lane, match(e.x, i0 + lane));
     }
     cluster.sync();   // the list is written, and hist may be again
   }
@@ -242,9 +254,9 @@ struct Cols {
 // entries long, and run by run the loads would wait for one another.
 template <typename T, bool VEC, bool ADD, int CHUNK>
 __global__ void __launch_bounds__(256)
-sorted_rows_kernel(const unsigned* __restrict__ keys, const unsigned* __restrict__ pos,
-                   long long n, unsigned V, const T* __restrict__ dout, int C, FastDiv slabs,
-                   unsigned tasks, T* grad, float scale, float* __restrict__ part) {
+sorted_rows_kernel(const uint2* __restrict__ list, long long n, unsigned V,
+                   const T* __restrict__ dout, int C, FastDiv slabs, unsigned tasks, T* grad,
+                   float scale, float* __restrict__ part, unsigned* __restrict__ open_runs) {
   ::msb::pdl_begin();
   const int lane = threadIdx.x & 31;
   const unsigned task = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -254,10 +266,10 @@ sorted_rows_kernel(const unsigned* __restrict__ keys, const unsigned* __restrict
   const int c0 = (int)(task - j * slabs.d) * 256 + (VEC ? lane * 8 : lane);
   const int len = (int)min((long long)CHUNK, n - first);
   // lane l: entry l's token; what comes before and behind the chunk
-  const unsigned my_key = lane < len ? keys[first + lane] : V;
-  const unsigned my_pos = lane < len ? pos[first + lane] : 0u;
-  const unsigned prev = first > 0 ? keys[first - 1] : V;
-  const unsigned next = first + CHUNK < n ? keys[first + CHUNK] : V;
+  const uint2 entry = lane < len ? list[first + lane] : make_uint2(V, 0u);
+  const unsigned my_key = entry.x, my_pos = entry.y;
+  const unsigned prev = first > 0 ? list[first - 1].x : V;
+  const unsigned next = first + CHUNK < n ? list[first + CHUNK].x : V;
   unsigned behind = __shfl_down_sync(0xffffffffu, my_key, 1);   // the key after each entry
   if (lane == CHUNK - 1) behind = next;
   // entries that are tokens, and those that end a run inside the chunk
@@ -303,6 +315,7 @@ sorted_rows_kernel(const unsigned* __restrict__ keys, const unsigned* __restrict
         }
         Cols<T, VEC>::store(grad + (long long)k * C, c0, C, f);
       } else {   // a part: slot 0 continues the chunk before, slot 1 begins here
+        if (!(in_head >> e & 1) && c0 == 0) open_runs[1 + atomicAdd(open_runs, 1u)] = j;
         float* d = part + ((long long)j * 2 + (in_head >> e & 1 ? 0 : 1)) * C;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -316,65 +329,65 @@ sorted_rows_kernel(const unsigned* __restrict__ keys, const unsigned* __restrict
   }
 }
 
-// Block j adds up the run that begins in chunk j and goes on behind it: its
-// threads look for the end together, then eight groups of warps add the parts
-// of an eighth of the chunks each, and the eight sums are added in order.
+// Adds up the runs that go on behind the chunk they begin in (listed in any
+// order by the kernel above; each is a task of its own, 128 columns at a time).
+// A block looks for the run's last chunk with all its threads, its eight warps
+// add the parts of an eighth of the chunks each, and the eight sums are added
+// in order.  V4: C is a multiple of 4.
 constexpr int kRunThreads = 256;
-constexpr int kRunGroups = 8;
-template <typename T, bool ADD, int CHUNK>
+constexpr int kRunWarps = kRunThreads / 32;
+constexpr int kRunCols = 128;
+template <typename T, bool ADD, bool V4, int CHUNK>
 __global__ void __launch_bounds__(kRunThreads)
-sorted_runs_kernel(const unsigned* __restrict__ keys, long long n, unsigned V,
-                   const float* __restrict__ part, int C, T* grad, float scale) {
+sorted_runs_kernel(const uint2* __restrict__ list, long long n, const float* __restrict__ part,
+                   int C, FastDiv slabs, T* grad, float scale,
+                   const unsigned* __restrict__ open_runs) {
   ::msb::pdl_begin();
-  __shared__ float sums[kRunGroups][128];
-  const long long j = blockIdx.x, first = j * CHUNK, after = first + CHUNK;
-  if (after >= n) return;
-  const unsigned key = keys[after];
-  if (key >= V || keys[after - 1] != key) return;          // nothing goes on
-  if (keys[first] == key && j > 0 && keys[first - 1] == key) return;   // began earlier
-  long long count = 1;   // chunks that begin with this token, from j + 1 on
-  for (;;) {
-    const long long at = (j + 1 + count + threadIdx.x) * CHUNK;
-    const int more = __syncthreads_count(at < n && keys[at] == key);
-    count += more;
-    if (more < kRunThreads) break;
-  }
-  T* g = grad + (long long)key * C;
-  const float* p0 = part + (j * 2 + 1) * C;
-  const float* p1 = part + (j + 1) * 2 * C;
-  if (count <= 2 * kRunGroups) {   // few parts: a thread a column
-    for (int c = threadIdx.x; c < C; c += kRunThreads) {
-      float a = p0[c];
-#pragma unroll 4
-      for (int i = 0; i < (int)count; ++i) a += p1[(long long)i * 2 * C + c];
-      g[c] = from_f32<T>(fmaf(a, scale, ADD ? to_f32(g[c]) : 0.f));
-    }
-    return;
-  }
+  __shared__ float4 sums[kRunWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long each = (count + kRunGroups - 1) / kRunGroups;
-  const long long i0 = min(count, each * warp), i1 = min(count, i0 + each);
-  for (int c0 = 0; c0 < C; c0 += 128) {
-    float a[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (long long i = i0; i < i1; ++i) {
+  const unsigned tasks = open_runs[0] * slabs.d;
+  for (unsigned task = blockIdx.x; task < tasks; task += gridDim.x) {
+    const unsigned run = slabs.div(task);
+    const long long j = open_runs[1 + run];
+    const int c = (int)(task - run * slabs.d) * kRunCols + lane * 4;
+    const unsigned key = list[j * CHUNK + CHUNK - 1].x;
+    long long count = 1;   // chunks that begin with this token, from j + 1 on
+    for (;;) {
+      const long long at = (j + 1 + count + threadIdx.x) * CHUNK;
+      const int more = __syncthreads_count(at < n && list[at].x == key);
+      count += more;
+      if (more < kRunThreads) break;
+    }
+    const float* p0 = part + (j * 2 + 1) * C;
+    const float* p1 = part + (j + 1) * 2 * C;
+    auto load = [&](const float* row) {
+      if (V4) return c < C ? *reinterpret_cast<const float4*>(row + c) : make_float4(0, 0, 0, 0);
+      return make_float4(c < C ? row[c] : 0.f, c + 1 < C ? row[c + 1] : 0.f,
+                         c + 2 < C ? row[c + 2] : 0.f, c + 3 < C ? row[c + 3] : 0.f);
+    };
+    const int each = (int)((count + kRunWarps - 1) / kRunWarps);
+    const int i0 = min((int)count, each * warp), i1 = min((int)count, i0 + each);
+    float4 a = warp == 0 ? load(p0) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int i = i0; i < i1; ++i) {
+      const float4 v = load(p1 + (long long)i * 2 * C);
+      a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+    }
+    sums[warp][lane] = a;
+    __syncthreads();
+    if (warp == 0) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int c = c0 + lane + 32 * k;
-        if (c < C) a[k] += p1[i * 2 * C + c];
+      for (int w = 1; w < kRunWarps; ++w) {
+        const float4 v = sums[w][lane];
+        a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
       }
-    }
-    __syncthreads();
+      T* g = grad + (long long)key * C + c;
+      const float f[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) sums[warp][lane + 32 * k] = a[k];
-    __syncthreads();
-    const int c = c0 + threadIdx.x;
-    if (threadIdx.x < 128 && c < C) {
-      float s = p0[c];
-#pragma unroll
-      for (int w = 0; w < kRunGroups; ++w) s += sums[w][threadIdx.x];
-      g[c] = from_f32<T>(fmaf(s, scale, ADD ? to_f32(g[c]) : 0.f));
+      for (int k = 0; k < 4; ++k)
+        if (c + k < C) g[k] = from_f32<T>(fmaf(f[k], scale, ADD ? to_f32(g[k]) : 0.f));
     }
+    __syncthreads();   // sums may be written again
   }
 }
 
@@ -404,9 +417,26 @@ void scaled_embedding_fwd(const long long* idx, const void* w, void* out, long l
   MSB_CHECK_LAUNCH("scaled_embedding_fwd");
 }
 
+// two lists of n entries, the number of open runs and the runs, the parts
+struct Workspace {
+  uint2 *a, *b;
+  unsigned* open_runs;
+  float* part;
+  long long words;
+  Workspace(unsigned* ws, long long n, long long chunks, int C) {
+    const long long runs = (chunks + 4) / 4 * 4;   // 1 + chunks, the parts 16-byte aligned
+    const long long lists = (4 * n + 3) / 4 * 4;
+    a = reinterpret_cast<uint2*>(ws);
+    b = reinterpret_cast<uint2*>(ws + 2 * n);
+    open_runs = ws + lists;
+    part = reinterpret_cast<float*>(ws + lists + runs);
+    words = lists + runs + chunks * 2 * C;
+  }
+};
+
 long long scaled_embedding_ws(long long n, int C) {
   const int chunk = chunk_of(n, (C + 255) / 256);
-  return 4 * n + (n + chunk - 1) / chunk * 2 * C;
+  return Workspace(nullptr, n, (n + chunk - 1) / chunk, C).words;
 }
 
 void scaled_embedding_bwd(const void* dout, const long long* idx, void* grad, bool accumulate,
@@ -418,8 +448,9 @@ void scaled_embedding_bwd(const void* dout, const long long* idx, void* grad, bo
   const int passes = n > 0 ? (total_bits + kDigit - 1) / kDigit : 0;
   // at least 2: a warp's counters are then whole vectors
   const int bits = passes > 0 && total_bits > 2 ? (total_bits + passes - 1) / passes : 2;
-  unsigned *ka = ws, *pa = ws + n, *kb = ws + 2 * n, *pb = ws + 3 * n;
-  float* part = reinterpret_cast<float*>(ws + 4 * n);
+  const int slabs = (C + 255) / 256, chunk = chunk_of(n, slabs);
+  const long long chunks = (n + chunk - 1) / chunk;
+  const Workspace w(ws, n, chunks, C);
   unsigned R = 1;
   while (R < kMaxCluster && (long long)R * kSortThreads < n) R *= 2;
   const size_t smem = sizeof(unsigned) * kSortWarps << bits;
@@ -432,40 +463,35 @@ void scaled_embedding_bwd(const void* dout, const long long* idx, void* grad, bo
   const unsigned extra = (unsigned)((blocks + R - 1) / R * R);
   if (n == 0 && extra == 0) return;
   launch_cluster(R, sort_tokens_kernel, R + extra, kSortThreads, smem, st, idx, n, V, padding,
-                 passes, bits, ka, pa, kb, pb, (uint4*)grad, fill_n, (int)(bytes % 16));
+                 passes, bits, w.a, w.b, w.open_runs, (uint4*)grad, fill_n, (int)(bytes % 16));
   if (n == 0) return;
-  const unsigned* keys = passes & 1 ? ka : kb;
-  const unsigned* pos = passes & 1 ? pa : pb;
-  const int slabs = (C + 255) / 256, chunk = chunk_of(n, slabs);
-  const long long chunks = (n + chunk - 1) / chunk;
+  const uint2* list = passes & 1 ? w.a : w.b;
   MSB_DISPATCH_FLOAT(dtype, T, {
     const bool vec = C % 8 == 0 && aligned16(dout) && aligned16(grad);
     const long long tasks = chunks * slabs;
     auto rows = [&](auto* kernel) {
-      launch(kernel, (unsigned)((tasks + 7) / 8), 256, 0, st, keys, pos, n, (unsigned)V,
-             (const T*)dout, C, FastDiv(slabs), (unsigned)tasks, (T*)grad, scale, part);
+      launch(kernel, (unsigned)((tasks + 7) / 8), 256, 0, st, list, n, (unsigned)V,
+             (const T*)dout, C, FastDiv(slabs), (unsigned)tasks, (T*)grad, scale, w.part,
+             w.open_runs);
     };
     auto runs = [&](auto* kernel) {
+      const int cols = (C + kRunCols - 1) / kRunCols;
       if (chunks > 1)
-        launch(kernel, (unsigned)chunks, kRunThreads, 0, st, keys, n, (unsigned)V, part, C,
-               (T*)grad, scale);
+        launch(kernel, grid_for(chunks * cols, 1, kNumSMs * 8), kRunThreads, 0, st, list, n, w.part,
+               C, FastDiv(cols), (T*)grad, scale, w.open_runs);
     };
-    if (chunk == 8) {
-      if (accumulate) {
-        vec ? rows(sorted_rows_kernel<T, true, true, 8>) : rows(sorted_rows_kernel<T, false, true, 8>);
-        runs(sorted_runs_kernel<T, true, 8>);
-      } else {
-        vec ? rows(sorted_rows_kernel<T, true, false, 8>) : rows(sorted_rows_kernel<T, false, false, 8>);
-        runs(sorted_runs_kernel<T, false, 8>);
-      }
+    auto go = [&](auto add, auto size) {
+      constexpr bool A = decltype(add)::value;
+      constexpr int N = decltype(size)::value;
+      vec ? rows(sorted_rows_kernel<T, true, A, N>) : rows(sorted_rows_kernel<T, false, A, N>);
+      C % 4 == 0 ? runs(sorted_runs_kernel<T, A, true, N>) : runs(sorted_runs_kernel<T, A, false, N>);
+    };
+    using Short = std::integral_constant<int, 8>;
+    using Long = std::integral_constant<int, 32>;
+    if (accumulate) {
+      chunk == 8 ? go(std::true_type{}, Short{}) : go(std::true_type{}, Long{});
     } else {
-      if (accumulate) {
-        vec ? rows(sorted_rows_kernel<T, true, true, 32>) : rows(sorted_rows_kernel<T, false, true, 32>);
-        runs(sorted_runs_kernel<T, true, 32>);
-      } else {
-        vec ? rows(sorted_rows_kernel<T, true, false, 32>) : rows(sorted_rows_kernel<T, false, false, 32>);
-        runs(sorted_runs_kernel<T, false, 32>);
-      }
+      chunk == 8 ? go(std::false_type{}, Short{}) : go(std::false_type{}, Long{});
     }
   });
   MSB_CHECK_LAUNCH("scaled_embedding_bwd");
