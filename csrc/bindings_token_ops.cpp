@@ -198,30 +198,36 @@ at::Tensor logprob_bwd(const at::Tensor& logits, const at::Tensor& tokens, const
 }
 
 // ------------------------------------------------------- scaled embedding
-at::Tensor scaled_embedding_fwd(const at::Tensor& idx, const at::Tensor& weight, double scale) {
+// (out, list): with `sort`, the tokens' list for the backward, else none
+std::tuple<at::Tensor, OptT> scaled_embedding_fwd(const at::Tensor& idx, const at::Tensor& weight,
+                                                  double scale, int64_t padding, bool sort) {
   check_contig(weight, "weight");
   check_matrix(weight, "weight");
-  const long long* tok = tokens_of(idx, idx.numel(), weight);
-  const int64_t V = weight.size(0), C = weight.size(1);
-  TORCH_CHECK(V > 0 && V < (1LL << 31), "the table must have between 1 and 2^31 - 1 rows");
+  const int64_t n = idx.numel(), V = weight.size(0), C = weight.size(1);
+  const long long* tok = tokens_of(idx, n, weight);
+  TORCH_CHECK(V > 0 && V < (1LL << 31) && n < (1LL << 31) && C < (1LL << 30) &&
+                  n * ((C + 255) / 256) < (1LL << 34), "too large");
   c10::cuda::CUDAGuard g(weight.device());
   auto shape = idx.sizes().vec();
   shape.push_back(C);
   at::Tensor out = at::empty(shape, weight.options());
-  msb::scaled_embedding_fwd(tok, weight.data_ptr(), out.data_ptr(), idx.numel(), (int)C, V,
-                            (float)scale, dtype_code(weight), stream_of(weight));
-  return out;
+  OptT list;
+  if (sort) list = at::empty({4 * n}, weight.options().dtype(at::kInt));
+  msb::scaled_embedding_fwd(tok, weight.data_ptr(), out.data_ptr(), n, (int)C, V, (float)scale,
+                            padding, sort ? (unsigned*)list->data_ptr<int>() : nullptr,
+                            dtype_code(weight), stream_of(weight));
+  return {out, list};
 }
 
 // the gradient added into `sink` [V, C], or, without one, as a new tensor
-at::Tensor scaled_embedding_bwd(const at::Tensor& dout, const at::Tensor& idx, int64_t V,
-                                int64_t padding, double scale, const OptT& sink) {
+at::Tensor scaled_embedding_bwd(const at::Tensor& dout, const at::Tensor& list, int64_t V,
+                                double scale, const OptT& sink) {
   check_contig(dout, "dout");
-  const int64_t n = idx.numel(), C = dout.size(-1);
-  TORCH_CHECK(dout.dim() >= 1 && C > 0 && dout.numel() == n * C, "dout: [tokens, C]");
-  TORCH_CHECK(V > 0 && V < (1LL << 31) && n < (1LL << 31) && C < (1LL << 30) &&
-                  n * ((C + 255) / 256) < (1LL << 34), "too large");
-  const long long* tok = tokens_of(idx, n, dout);
+  check_contig(list, "list");
+  const int64_t C = dout.size(-1), n = list.numel() / 4;
+  TORCH_CHECK(list.scalar_type() == at::kInt && dout.dim() >= 1 && C > 0 &&
+                  dout.numel() == n * C && list.device() == dout.device(),
+              "dout: [tokens, C], with the list of its lookup");
   c10::cuda::CUDAGuard g(dout.device());
   at::Tensor grad;
   if (given(sink)) {
@@ -231,12 +237,12 @@ at::Tensor scaled_embedding_bwd(const at::Tensor& dout, const at::Tensor& idx, i
                 "sink: a [V, C] gradient of dout's type");
     grad = *sink;
   } else {
-    grad = at::empty({V, C}, dout.options());   // cleared beside the sorting
+    grad = at::empty({V, C}, dout.options());
   }
   at::Tensor ws = at::empty({msb::scaled_embedding_ws(n, (int)C)}, dout.options().dtype(at::kInt));
-  msb::scaled_embedding_bwd(dout.data_ptr(), tok, grad.data_ptr(), given(sink),
-                            reinterpret_cast<unsigned*>(ws.data_ptr<int>()), n, (int)C, V, padding,
-                            (float)scale, dtype_code(dout), stream_of(dout));
+  msb::scaled_embedding_bwd(dout.data_ptr(), (const unsigned*)list.data_ptr<int>(),
+                            grad.data_ptr(), given(sink), (unsigned*)ws.data_ptr<int>(), n, (int)C,
+                            V, (float)scale, dtype_code(dout), stream_of(dout));
   return grad;
 }
 

@@ -2,16 +2,16 @@
 //
 //   out[i] = scale * W[idx_i]        dW[v] = scale * sum over {i : idx_i = v} of dout[i]
 //
-// The sum of a row is taken in fp32 in an order that depends on idx alone:
-// the positions are sorted by token (stable, so ascending within a token), the
-// sorted list is cut into chunks of 8 or 32 entries, and every run of one token is
-// summed front to back inside a chunk; a run that crosses chunks leaves one
-// fp32 partial per chunk, added up in chunk order.  No atomics touch values,
-// so the gradient is the same from run to run, and no [V, C] accumulator is
-// kept.
+// The sum of a row is taken in fp32 in an order that depends on idx alone: the
+// positions are sorted by token (stable, so ascending within a token), the
+// sorted list is cut into chunks of 8 or 32 entries, and every run of one token
+// is summed front to back inside a chunk; a run that crosses chunks leaves one
+// fp32 partial per chunk, added up in chunk order.  No atomics touch values, so
+// the gradient is the same from run to run, and no [V, C] accumulator is kept.
 //
-// Tokens outside [0, V) read as a zero row; they and the padding token get no
-// gradient (key V, sorted behind all others).
+// The lookup sorts for the backward pass on one cluster while the other SMs
+// gather.  Tokens outside [0, V) read as a zero row; they and the padding token
+// get no gradient (key V, sorted behind all others).
 #include <cooperative_groups.h>
 
 #include <utility>
@@ -35,15 +35,14 @@ constexpr int kMaxCluster = 8;
 constexpr int kHeld = 4;            // entries a lane keeps in registers over a pass
 constexpr int kRows = 8;            // rows in flight in the sum kernel
 
-// VEC: eight columns a thread (width a multiple of 8, 16-byte aligned table)
+// out = scale * w[idx], from thread `first` of `threads` on.  VEC: eight columns a
+// thread (width a multiple of 8, 16-byte aligned table).
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256)
-scaled_embedding_fwd_kernel(const long long* __restrict__ idx, const T* __restrict__ w,
-                            T* __restrict__ out, unsigned total, FastDiv per, int C, long long V,
-                            float scale) {
-  ::msb::pdl_begin();
-  for (unsigned i = blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += gridDim.x * blockDim.x) {
+__device__ __forceinline__ void lookup(const long long* __restrict__ idx,
+                                       const T* __restrict__ w, T* __restrict__ out,
+                                       unsigned total, const FastDiv& per, int C, long long V,
+                                       float scale, unsigned first, unsigned threads) {
+  for (unsigned i = first; i < total; i += threads) {
     const unsigned m = per.div(i);
     const int c = (int)(i - m * per.d) * (VEC ? 8 : 1);
     const long long t = idx[m];
@@ -61,9 +60,16 @@ scaled_embedding_fwd_kernel(const long long* __restrict__ idx, const T* __restri
   }
 }
 
-// The first cluster sorts (token, position) by token, 9 bits or fewer a pass;
-// the others meanwhile clear the gradient (fill_n vectors of 16 bytes, and
-// fill_tail bytes behind them), where it is a new one.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+lookup_kernel(const long long* __restrict__ idx, const T* __restrict__ w, T* __restrict__ out,
+              unsigned total, FastDiv per, int C, long long V, float scale) {
+  ::msb::pdl_begin();
+  lookup<T, VEC>(idx, w, out, total, per, C, V, scale, blockIdx.x * blockDim.x + threadIdx.x,
+                 gridDim.x * blockDim.x);
+}
+
+// Sorts (token, position) by token on one cluster, 9 bits or fewer a pass.
 //
 // Every warp of the cluster owns one contiguous piece of the list.  A pass
 // counts the digits of each warp's piece, turns the counts into places (over
@@ -72,26 +78,15 @@ scaled_embedding_fwd_kernel(const long long* __restrict__ idx, const T* __restri
 // place, warp by warp in order, lanes with the same digit ranked by ballots on
 // its bits (__match_any_sync took seven times as long): stable by construction.
 // The cluster barrier orders the passes.  What bounds it is the latency of its
-// steps: 16384 tokens of 50257 take SORT16K us.
-__global__ void __launch_bounds__(kSortThreads)
-sort_tokens_kernel(const long long* __restrict__ idx, long long n, long long V,
-                   long long padding, int passes, int bits, uint2* list_a, uint2* list_b,
-                   unsigned* open_runs, uint4* fill, long long fill_n, int fill_tail) {
-  ::msb::pdl_begin();
+// steps: 16384 tokens of 50257 take 13 us.
+__device__ __forceinline__ void sort_tokens(const long long* __restrict__ idx, long long n,
+                                            long long V, long long padding, int passes, int bits,
+                                            uint2* list_a, uint2* list_b) {
   extern __shared__ unsigned cnt[];   // [kSortWarps][1 << bits]
   __shared__ unsigned hist[kMaxCluster][kBins], base[kBins], wsum[kSortWarps], quarter[4][kBins];
   cg::cluster_group cluster = cg::this_cluster();
   const unsigned q = cluster.block_rank(), R = cluster.num_blocks();
-  if (blockIdx.x >= R) {
-    const long long threads = (long long)(gridDim.x - R) * kSortThreads;
-    const long long first = (long long)(blockIdx.x - R) * kSortThreads + threadIdx.x;
-    for (long long i = first; i < fill_n; i += threads) fill[i] = make_uint4(0, 0, 0, 0);
-    if (first < fill_tail) reinterpret_cast<unsigned char*>(fill + fill_n)[first] = 0;
-    return;
-  }
-  if (passes == 0) return;
   auto started = cluster.barrier_arrive();   // waited for before another block's memory is written
-  if (blockIdx.x == 0 && threadIdx.x == 0) *open_runs = 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int bins = 1 << bits;
   const unsigned ones = (unsigned)bins - 1u, below = (1u << lane) - 1u;
@@ -207,6 +202,24 @@ sort_tokens_kernel(const long long* __restrict__ idx, long long n, long long V,
   }
 }
 
+// The first cluster sorts, the others gather.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kSortThreads)
+lookup_sort_kernel(const long long* __restrict__ idx, const T* __restrict__ w,
+                   T* __restrict__ out, unsigned total, FastDiv per, int C, long long V,
+                   float scale, long long n, long long padding, int passes, int bits,
+                   uint2* list_a, uint2* list_b) {
+  ::msb::pdl_begin();
+  const unsigned R = cg::this_cluster().num_blocks();
+  if (blockIdx.x < R) {
+    sort_tokens(idx, n, V, padding, passes, bits, list_a, list_b);
+  } else {
+    lookup<T, VEC>(idx, w, out, total, per, C, V, scale,
+                   (blockIdx.x - R) * kSortThreads + threadIdx.x,
+                   (gridDim.x - R) * kSortThreads);
+  }
+}
+
 // Eight columns of a row as a lane holds them: packed while in flight.  VEC:
 // adjacent columns from c0 on; otherwise c0 + 32 k, for widths and addresses that
 // do not allow 16-byte accesses.
@@ -248,16 +261,67 @@ struct Cols {
   }
 };
 
+// Clears the rows of a unit of `unit` table rows that no entry of the list names.
+constexpr int kUnitRows = 1024;
+template <typename T, bool VEC>
+__device__ __forceinline__ void clear_unit(const uint2* __restrict__ list, long long n,
+                                           long long V, int C, T* grad, long long u, int unit) {
+  __shared__ unsigned char named[kUnitRows];
+  const long long v0 = u * unit, v1 = min(V, v0 + unit);
+  for (int i = threadIdx.x; i < unit; i += blockDim.x) named[i] = 0;
+  // the first entry that is not before v0: all threads probe, 256 places at a time
+  long long lo = 0, hi = n;
+  while (lo < hi) {
+    const long long step = (hi - lo + blockDim.x - 1) / blockDim.x;
+    const long long at = lo + threadIdx.x * step;
+    const int before = __syncthreads_count(at < hi && list[at].x < v0);
+    if (before == 0) break;             // list[lo] is not before v0
+    hi = min(hi, lo + before * step);   // nor is list[lo + before * step]
+    lo += (before - 1) * step + 1;
+  }
+  for (;;) {   // mark the unit's
+    const long long at = lo + threadIdx.x;
+    const unsigned k = at < n ? list[at].x : 0xffffffffu;
+    if (k < v1) named[k - v0] = 1;
+    if (__syncthreads_count(k < v1) < (int)blockDim.x) break;
+    lo += blockDim.x;
+  }
+  T* g = grad + v0 * C;
+  if (VEC) {
+    constexpr int N = 16 / sizeof(T);
+    const int per = C / N, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int r = warp; r < v1 - v0; r += blockDim.x >> 5) {
+      if (named[r]) continue;
+      uint4* p = reinterpret_cast<uint4*>(g + (long long)r * C);
+      for (int i = lane; i < per; i += 32) p[i] = make_uint4(0, 0, 0, 0);
+    }
+  } else {
+    for (int r = 0; r < v1 - v0; ++r) {
+      if (named[r]) continue;
+      for (int c = threadIdx.x; c < C; c += blockDim.x) g[(long long)r * C + c] = from_f32<T>(0.f);
+    }
+  }
+}
+
 // A warp sums a chunk of CHUNK sorted entries over 256 columns.  The rows of
 // eight entries, and the gradient rows that their sums are added to, are loaded
 // before any is used, whatever runs they belong to: most runs are one or two
-// entries long, and run by run the loads would wait for one another.
+// entries long, and run by run the loads would wait for one another.  open[j]:
+// a run begins in chunk j and goes on behind it.
+//
+// ADD: the sums are added to the rows.  Otherwise the gradient is a new one, and
+// the blocks behind the first `row_blocks` clear the rows of no token meanwhile.
 template <typename T, bool VEC, bool ADD, int CHUNK>
 __global__ void __launch_bounds__(256)
 sorted_rows_kernel(const uint2* __restrict__ list, long long n, unsigned V,
                    const T* __restrict__ dout, int C, FastDiv slabs, unsigned tasks, T* grad,
-                   float scale, float* __restrict__ part, unsigned* __restrict__ open_runs) {
+                   float scale, float* __restrict__ part, unsigned char* __restrict__ open,
+                   unsigned row_blocks, int unit) {
   ::msb::pdl_begin();
+  if (!ADD && blockIdx.x >= row_blocks) {
+    clear_unit<T, VEC>(list, n, V, C, grad, blockIdx.x - row_blocks, unit);
+    return;
+  }
   const int lane = threadIdx.x & 31;
   const unsigned task = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (task >= tasks) return;
@@ -275,11 +339,13 @@ sorted_rows_kernel(const uint2* __restrict__ list, long long n, unsigned V,
   // entries that are tokens, and those that end a run inside the chunk
   const unsigned live = __ballot_sync(0xffffffffu, lane < len && my_key < V);
   const unsigned ends = __ballot_sync(0xffffffffu, lane < len && my_key < V && behind != my_key);
+  if (c0 == 0) open[j] = live >> (CHUNK - 1) & 1 && !(ends >> (CHUNK - 1) & 1);   // goes on
   if (live == 0) return;
   const unsigned key0 = __shfl_sync(0xffffffffu, my_key, 0);
   const int head = prev == key0 ? __ffs(~__ballot_sync(0xffffffffu, my_key == key0)) - 1 : 0;
   // `head` entries, when not 0, continue the run of the chunk before (32 of 32: -1)
   const unsigned in_head = prev != key0 ? 0u : head < 0 ? ~0u : (1u << head) - 1u;
+  if (c0 == 0 && (in_head >> (CHUNK - 1) & 1)) open[j] = 0;   // but began earlier
   float a[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 1
   for (int e0 = 0; e0 < CHUNK; e0 += kRows) {
@@ -315,7 +381,6 @@ sorted_rows_kernel(const uint2* __restrict__ list, long long n, unsigned V,
         }
         Cols<T, VEC>::store(grad + (long long)k * C, c0, C, f);
       } else {   // a part: slot 0 continues the chunk before, slot 1 begins here
-        if (!(in_head >> e & 1) && c0 == 0) open_runs[1 + atomicAdd(open_runs, 1u)] = j;
         float* d = part + ((long long)j * 2 + (in_head >> e & 1 ? 0 : 1)) * C;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -329,50 +394,82 @@ sorted_rows_kernel(const uint2* __restrict__ list, long long n, unsigned V,
   }
 }
 
-// Adds up the runs that go on behind the chunk they begin in (listed in any
-// order by the kernel above; each is a task of its own, 128 columns at a time).
-// A block looks for the run's last chunk with all its threads, its eight warps
-// add the parts of an eighth of the chunks each, and the eight sums are added
-// in order.  V4: C is a multiple of 4.
+// Adds up the runs that go on behind the chunk they begin in.  A block has 32
+// chunks and 128 columns; each of its warps takes every eighth open run among
+// them and adds its parts in order, and runs of more than kLongRun parts, left
+// for last, are added by the eight warps together, an eighth of the parts each,
+// the eight sums in order.  V4: C is a multiple of 4.
 constexpr int kRunThreads = 256;
 constexpr int kRunWarps = kRunThreads / 32;
 constexpr int kRunCols = 128;
+constexpr int kLongRun = 24;
+static_assert(kLongRun < 32, "a warp's one look finds the end of a short run");
 template <typename T, bool ADD, bool V4, int CHUNK>
 __global__ void __launch_bounds__(kRunThreads)
 sorted_runs_kernel(const uint2* __restrict__ list, long long n, const float* __restrict__ part,
-                   int C, FastDiv slabs, T* grad, float scale,
-                   const unsigned* __restrict__ open_runs) {
+                   int C, long long chunks, FastDiv slabs, T* grad, float scale,
+                   const unsigned char* __restrict__ open) {
   ::msb::pdl_begin();
   __shared__ float4 sums[kRunWarps][32];
+  __shared__ unsigned is_long;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const unsigned tasks = open_runs[0] * slabs.d;
-  for (unsigned task = blockIdx.x; task < tasks; task += gridDim.x) {
-    const unsigned run = slabs.div(task);
-    const long long j = open_runs[1 + run];
-    const int c = (int)(task - run * slabs.d) * kRunCols + lane * 4;
+  const unsigned group = slabs.div(blockIdx.x);
+  const int c = (int)(blockIdx.x - group * slabs.d) * kRunCols + lane * 4;
+  const long long j0 = (long long)group * 32;
+  unsigned todo = __ballot_sync(0xffffffffu, j0 + lane < chunks && open[j0 + lane]);
+  if (todo == 0) return;   // in all warps alike
+  if (threadIdx.x == 0) is_long = 0;
+  __syncthreads();
+  auto load = [&](const float* row) {
+    if (V4) return c < C ? *reinterpret_cast<const float4*>(row + c) : make_float4(0, 0, 0, 0);
+    return make_float4(c < C ? row[c] : 0.f, c + 1 < C ? row[c + 1] : 0.f,
+                       c + 2 < C ? row[c + 2] : 0.f, c + 3 < C ? row[c + 3] : 0.f);
+  };
+  auto add_parts = [&](float4& a, long long j, int i0, int i1) {   // of chunks j + 1 + i
+    const float* p = part + (j + 1) * 2 * C;
+#pragma unroll 8
+    for (int i = i0; i < i1; ++i) {
+      const float4 v = load(p + (long long)i * 2 * C);
+      a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+    }
+  };
+  auto put = [&](const float4& a, unsigned key) {
+    T* g = grad + (long long)key * C + c;
+    const float f[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c + k < C) g[k] = from_f32<T>(fmaf(f[k], scale, ADD ? to_f32(g[k]) : 0.f));
+  };
+  for (int t = 0; todo != 0; ++t, todo &= todo - 1) {
+    if (t % kRunWarps != warp) continue;
+    const int b = __ffs(todo) - 1;
+    const long long j = j0 + b, at = (j + 1 + lane) * CHUNK;   // the chunks behind j
     const unsigned key = list[j * CHUNK + CHUNK - 1].x;
-    long long count = 1;   // chunks that begin with this token, from j + 1 on
+    const unsigned other = ~__ballot_sync(0xffffffffu, at < n && list[at].x == key);
+    const int count = other == 0 ? 32 : __ffs(other) - 1;
+    if (count > kLongRun) {
+      if (lane == 0) atomicOr(&is_long, 1u << b);
+      continue;
+    }
+    float4 a = load(part + (j * 2 + 1) * C);
+    add_parts(a, j, 0, count);
+    put(a, key);
+  }
+  __syncthreads();
+  for (unsigned rest = is_long; rest != 0; rest &= rest - 1) {
+    const long long j = j0 + __ffs(rest) - 1;
+    const unsigned key = list[j * CHUNK + CHUNK - 1].x;
+    long long count = 0;
     for (;;) {
       const long long at = (j + 1 + count + threadIdx.x) * CHUNK;
       const int more = __syncthreads_count(at < n && list[at].x == key);
       count += more;
       if (more < kRunThreads) break;
     }
-    const float* p0 = part + (j * 2 + 1) * C;
-    const float* p1 = part + (j + 1) * 2 * C;
-    auto load = [&](const float* row) {
-      if (V4) return c < C ? *reinterpret_cast<const float4*>(row + c) : make_float4(0, 0, 0, 0);
-      return make_float4(c < C ? row[c] : 0.f, c + 1 < C ? row[c + 1] : 0.f,
-                         c + 2 < C ? row[c + 2] : 0.f, c + 3 < C ? row[c + 3] : 0.f);
-    };
     const int each = (int)((count + kRunWarps - 1) / kRunWarps);
     const int i0 = min((int)count, each * warp), i1 = min((int)count, i0 + each);
-    float4 a = warp == 0 ? load(p0) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int i = i0; i < i1; ++i) {
-      const float4 v = load(p1 + (long long)i * 2 * C);
-      a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
-    }
+    float4 a = warp == 0 ? load(part + (j * 2 + 1) * C) : make_float4(0.f, 0.f, 0.f, 0.f);
+    add_parts(a, j, i0, i1);
     sums[warp][lane] = a;
     __syncthreads();
     if (warp == 0) {
@@ -381,11 +478,7 @@ sorted_runs_kernel(const uint2* __restrict__ list, long long n, const float* __r
         const float4 v = sums[w][lane];
         a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
       }
-      T* g = grad + (long long)key * C + c;
-      const float f[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (c + k < C) g[k] = from_f32<T>(fmaf(f[k], scale, ADD ? to_f32(g[k]) : 0.f));
+      put(a, key);
     }
     __syncthreads();   // sums may be written again
   }
@@ -393,92 +486,89 @@ sorted_runs_kernel(const uint2* __restrict__ list, long long n, const float* __r
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Entries of a chunk: 8 while that makes no more than 2^18 tasks (the more warps,
+// Entries of a chunk: 8 while that makes no more than 2^15 tasks (the more warps,
 // the shorter their chains of loads), then 32 (fewer parts of cut runs).
-int chunk_of(long long n, int slabs) { return n * slabs <= (8LL << 18) ? 8 : 32; }
+int chunk_of(long long n, int C) { return n * ((C + 255) / 256) <= (8LL << 15) ? 8 : 32; }
 
 }  // namespace
 
+// the list that the backward needs is in the first 2 n words of `ws`, which has
+// 4 n (null: not wanted)
 void scaled_embedding_fwd(const long long* idx, const void* w, void* out, long long n, int C,
-                          long long V, float scale, int dtype, cudaStream_t st) {
+                          long long V, float scale, long long padding, unsigned* ws, int dtype,
+                          cudaStream_t st) {
+  if (n == 0) return;
   MSB_DISPATCH_FLOAT(dtype, T, {
     const bool vec = C % 8 == 0 && aligned16(w);
     const int per = vec ? C / 8 : C;
     const long long fit = (1LL << 30) / per, most = fit > 0 ? fit : 1;   // tokens a launch
     for (long long i = 0; i < n; i += most) {
       const unsigned total = (unsigned)((n - i < most ? n - i : most) * per);
+      if (ws != nullptr && i == 0) {
+        // tokens and V itself (no token) in as few passes of at most kDigit bits;
+        // at least 2: a warp's counters are then whole vectors
+        int total_bits = 2;
+        while ((V >> total_bits) != 0) ++total_bits;
+        const int passes = (total_bits + kDigit - 1) / kDigit;
+        const int bits = max(2, (total_bits + passes - 1) / passes);
+        unsigned R = 1;
+        while (R < kMaxCluster && (long long)R * kSortThreads < n) R *= 2;
+        const unsigned gather = (grid_for(total, kSortThreads, kNumSMs * 2) + R - 1) / R * R;
+        uint2 *a = (uint2*)ws, *b = (uint2*)(ws + 2 * n);
+        auto go = [&](auto* kernel) {
+          check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          (int)sizeof(unsigned) * kSortWarps * kBins),
+                     "lookup_sort smem");
+          launch_cluster(R, kernel, R + gather, kSortThreads, sizeof(unsigned) * kSortWarps << bits,
+                         st, idx, (const T*)w, (T*)out, total, FastDiv(per), C, V, scale, n,
+                         padding, passes, bits, passes & 1 ? a : b, passes & 1 ? b : a);
+        };
+        vec ? go(lookup_sort_kernel<T, true>) : go(lookup_sort_kernel<T, false>);
+        continue;
+      }
       auto go = [&](auto* kernel) {
         launch(kernel, grid_for(total, 256, kNumSMs * 16), 256, 0, st, idx + i, (const T*)w,
                (T*)out + i * C, total, FastDiv(per), C, V, scale);
       };
-      vec ? go(scaled_embedding_fwd_kernel<T, true>) : go(scaled_embedding_fwd_kernel<T, false>);
+      vec ? go(lookup_kernel<T, true>) : go(lookup_kernel<T, false>);
     }
   });
   MSB_CHECK_LAUNCH("scaled_embedding_fwd");
 }
 
-// two lists of n entries, the number of open runs and the runs, the parts
-struct Workspace {
-  uint2 *a, *b;
-  unsigned* open_runs;
-  float* part;
-  long long words;
-  Workspace(unsigned* ws, long long n, long long chunks, int C) {
-    const long long runs = (chunks + 4) / 4 * 4;   // 1 + chunks, the parts 16-byte aligned
-    const long long lists = (4 * n + 3) / 4 * 4;
-    a = reinterpret_cast<uint2*>(ws);
-    b = reinterpret_cast<uint2*>(ws + 2 * n);
-    open_runs = ws + lists;
-    part = reinterpret_cast<float*>(ws + lists + runs);
-    words = lists + runs + chunks * 2 * C;
-  }
-};
-
+// a flag a chunk, then the parts, 16-byte aligned
+static long long flag_words(long long chunks) { return (chunks + 15) / 16 * 4; }
 long long scaled_embedding_ws(long long n, int C) {
-  const int chunk = chunk_of(n, (C + 255) / 256);
-  return Workspace(nullptr, n, (n + chunk - 1) / chunk, C).words;
+  const long long chunk = chunk_of(n, C), chunks = (n + chunk - 1) / chunk;
+  return flag_words(chunks) + chunks * 2 * C;
 }
 
-void scaled_embedding_bwd(const void* dout, const long long* idx, void* grad, bool accumulate,
-                          unsigned* ws, long long n, int C, long long V, long long padding,
-                          float scale, int dtype, cudaStream_t st) {
-  // tokens and V itself (no token) in as few passes of at most kDigit bits
-  int total_bits = 1;
-  while ((V >> total_bits) != 0) ++total_bits;
-  const int passes = n > 0 ? (total_bits + kDigit - 1) / kDigit : 0;
-  // at least 2: a warp's counters are then whole vectors
-  const int bits = passes > 0 && total_bits > 2 ? (total_bits + passes - 1) / passes : 2;
-  const int slabs = (C + 255) / 256, chunk = chunk_of(n, slabs);
+void scaled_embedding_bwd(const void* dout, const unsigned* sorted, void* grad, bool accumulate,
+                          unsigned* ws, long long n, int C, long long V, float scale, int dtype,
+                          cudaStream_t st) {
+  const uint2* list = (const uint2*)sorted;
+  const int slabs = (C + 255) / 256, chunk = chunk_of(n, C);
   const long long chunks = (n + chunk - 1) / chunk;
-  const Workspace w(ws, n, chunks, C);
-  unsigned R = 1;
-  while (R < kMaxCluster && (long long)R * kSortThreads < n) R *= 2;
-  const size_t smem = sizeof(unsigned) * kSortWarps << bits;
-  check_cuda(cudaFuncSetAttribute(sort_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  (int)(sizeof(unsigned) * kSortWarps * kBins)), "sort_tokens smem");
-  const long long bytes = accumulate ? 0 : V * C * (dtype == kF32 ? 4 : 2);
-  // the clearing blocks: 16 vectors a thread, in whole clusters
-  const long long fill_n = bytes / 16;
-  const long long blocks = (fill_n + 16 * kSortThreads - 1) / (16 * kSortThreads) + (bytes % 16 != 0);
-  const unsigned extra = (unsigned)((blocks + R - 1) / R * R);
-  if (n == 0 && extra == 0) return;
-  launch_cluster(R, sort_tokens_kernel, R + extra, kSortThreads, smem, st, idx, n, V, padding,
-                 passes, bits, w.a, w.b, w.open_runs, (uint4*)grad, fill_n, (int)(bytes % 16));
-  if (n == 0) return;
-  const uint2* list = passes & 1 ? w.a : w.b;
+  unsigned char* open = (unsigned char*)ws;
+  float* part = (float*)(ws + flag_words(chunks));
   MSB_DISPATCH_FLOAT(dtype, T, {
     const bool vec = C % 8 == 0 && aligned16(dout) && aligned16(grad);
     const long long tasks = chunks * slabs;
+    const unsigned row_blocks = (unsigned)((tasks + 7) / 8);
+    // units of 256 KB to clear
+    const long long fit = (256LL << 10) / ((long long)C * sizeof(T));
+    const int unit = (int)(fit < 1 ? 1 : fit > kUnitRows ? kUnitRows : fit);
+    const unsigned units = accumulate ? 0 : (unsigned)((V + unit - 1) / unit);
     auto rows = [&](auto* kernel) {
-      launch(kernel, (unsigned)((tasks + 7) / 8), 256, 0, st, list, n, (unsigned)V,
-             (const T*)dout, C, FastDiv(slabs), (unsigned)tasks, (T*)grad, scale, w.part,
-             w.open_runs);
+      if (row_blocks + units > 0)
+        launch(kernel, row_blocks + units, 256, 0, st, list, n, (unsigned)V, (const T*)dout, C,
+               FastDiv(slabs), (unsigned)tasks, (T*)grad, scale, part, open, row_blocks, unit);
     };
     auto runs = [&](auto* kernel) {
       const int cols = (C + kRunCols - 1) / kRunCols;
       if (chunks > 1)
-        launch(kernel, grid_for(chunks * cols, 1, kNumSMs * 8), kRunThreads, 0, st, list, n, w.part,
-               C, FastDiv(cols), (T*)grad, scale, w.open_runs);
+        launch(kernel, (unsigned)((chunks + 31) / 32 * cols), kRunThreads, 0, st, list, n, part, C,
+               chunks, FastDiv(cols), (T*)grad, scale, open);
     };
     auto go = [&](auto add, auto size) {
       constexpr bool A = decltype(add)::value;

@@ -121,15 +121,18 @@ void logprob_bwd(const void* logits, long long ld, const long long* tok, long lo
                  float temperature, long long ignore_index, int k, const long long* top_tok,
                  const float* stats, const float* g_logp, const float* g_ent, const float* g_top,
                  void* dx, long long ld_dx, int dtype, cudaStream_t st);
-// embedding with scaling (embedding_sorted.cu); the backward writes all of grad
-// or, with `accumulate`, adds to the rows of the tokens that occur; it needs
-// scaled_embedding_ws words of scratch; padding < 0: none
+// embedding with scaling (embedding_sorted.cu).  The forward leaves the list of
+// its tokens, sorted, in the first 2 n of the 4 n words at `ws` (null: it does
+// not sort); padding < 0: none.  The backward reads that list and writes all of
+// grad or, with `accumulate`, adds to the rows of the tokens that occur; it needs
+// scaled_embedding_ws words of scratch.
 void scaled_embedding_fwd(const long long* idx, const void* w, void* out, long long n, int C,
-                          long long V, float scale, int dtype, cudaStream_t st);
+                          long long V, float scale, long long padding, unsigned* ws, int dtype,
+                          cudaStream_t st);
 long long scaled_embedding_ws(long long n, int C);
-void scaled_embedding_bwd(const void* dout, const long long* idx, void* grad, bool accumulate,
-                          unsigned* ws, long long n, int C, long long V, long long padding,
-                          float scale, int dtype, cudaStream_t st);
+void scaled_embedding_bwd(const void* dout, const unsigned* sorted, void* grad, bool accumulate,
+                          unsigned* ws, long long n, int C, long long V, float scale, int dtype,
+                          cudaStream_t st);
 // activations in 8 bits (pack8_kernels.cu): codes [rows, 32 * nb], scales [rows, nb],
 // nb = ceil(D / 32); swiglu8_*: rows of [gate (F) | up (F)], packed as 2 * rows rows of F
 void pack8(const void* x, long long ld, signed char* codes, unsigned char* scales, long long rows,

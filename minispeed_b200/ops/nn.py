@@ -819,27 +819,29 @@ def embedding(idx: torch.Tensor, wte: torch.Tensor, wpe: Optional[torch.Tensor] 
 class _ScaledEmbedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, idx, weight, scale, padding):
-        idx = idx.contiguous()
         if weight.is_cuda:
-            out = _C().scaled_embedding_fwd(idx, weight.contiguous(), scale)
+            # what backward needs of the tokens is their sorted list
+            out, kept = _C().scaled_embedding_fwd(idx.contiguous(), weight.contiguous(), scale,
+                                                  padding, ctx.needs_input_grad[1])
         else:
-            out = (F.embedding(idx, weight).float() * scale).to(weight.dtype)
-        ctx.save_for_backward(idx)
+            out, kept = (F.embedding(idx, weight).float() * scale).to(weight.dtype), idx
+        ctx.save_for_backward(kept)
         ctx.weight = weight
         ctx.args = (weight.shape[0], padding, scale)
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        (idx,) = ctx.saved_tensors
+        (kept,) = ctx.saved_tensors
         V, padding, scale = ctx.args
         sink = grad_sink(ctx.weight)
         if dout.is_cuda:
-            dw = _C().scaled_embedding_bwd(dout.contiguous(), idx, V, padding, scale, sink)
+            dw = _C().scaled_embedding_bwd(dout.contiguous(), kept, V, scale, sink)
             return None, None if sink is not None else dw, None, None
+        idx = kept.reshape(-1)
         rows = dout.reshape(idx.numel(), -1).float() * scale
-        rows = torch.where((idx.reshape(-1) == padding)[:, None], 0.0, rows)
-        dw = torch.zeros(V, dout.shape[-1]).index_add_(0, idx.reshape(-1), rows)
+        rows = torch.where((idx == padding)[:, None], 0.0, rows)
+        dw = torch.zeros(V, dout.shape[-1]).index_add_(0, idx, rows)
         return None, dw.to(dout.dtype), None, None
 
 
