@@ -31,9 +31,56 @@ constexpr int kSortThreads = 1024;
 constexpr int kDigit = 9;           // most bits of a sorting pass
 constexpr int kBins = 1 << kDigit;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 8;   // 16 blocks sort 16384 tokens in 12 us, but are not portable
 constexpr int kHeld = 4;            // entries a lane keeps in registers over a pass
-constexpr int kRows = 8;            // rows in flight in the sum kernel
+constexpr int kRows = 4;            // rows in flight in the sum kernel (8: 13.9 us for 16384 x 768, 4: 12.9)
+
+// Eight columns of a row as a lane holds them: packed while in flight.  VEC:
+// adjacent columns from c0 on; otherwise c0 + 32 k, for widths and addresses that
+// do not allow 16-byte accesses.
+template <typename T, bool VEC>
+struct Cols {
+  uint4 r[sizeof(T) == 4 ? 2 : 1];
+  T e[VEC ? 1 : 8];
+  __device__ __forceinline__ void load(const T* row, int c0, int C) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int k = 0; k < (int)(sizeof(T) == 4 ? 2 : 1); ++k)
+        r[k] = c0 < C ? reinterpret_cast<const uint4*>(row + c0)[k] : make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) e[k] = c0 + 32 * k < C ? row[c0 + 32 * k] : from_f32<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ void numbers(float (&f)[8]) const {
+    if constexpr (!VEC) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = to_f32(e[k]);
+    } else if constexpr (sizeof(T) == 2) {
+      unpack_u4<T>(r[0], f);
+    } else {
+      const uint4 a = r[0], b = r[sizeof(T) == 4 ? 1 : 0];
+      f[0] = __uint_as_float(a.x), f[1] = __uint_as_float(a.y), f[2] = __uint_as_float(a.z),
+      f[3] = __uint_as_float(a.w), f[4] = __uint_as_float(b.x), f[5] = __uint_as_float(b.y),
+      f[6] = __uint_as_float(b.z), f[7] = __uint_as_float(b.w);
+    }
+  }
+  static __device__ __forceinline__ void store(T* row, int c0, int C, const float (&f)[8]) {
+    if constexpr (!VEC) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (c0 + 32 * k < C) row[c0 + 32 * k] = from_f32<T>(f[k]);
+    } else {
+      if (c0 >= C) return;
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(row + c0) = pack_u4<T>(f);
+      } else {
+        reinterpret_cast<float4*>(row + c0)[0] = make_float4(f[0], f[1], f[2], f[3]);
+        reinterpret_cast<float4*>(row + c0)[1] = make_float4(f[4], f[5], f[6], f[7]);
+      }
+    }
+  }
+};
 
 // out = scale * w[idx], from thread `first` of `threads` on.  VEC: eight columns a
 // thread (width a multiple of 8, 16-byte aligned table).
@@ -42,20 +89,37 @@ __device__ __forceinline__ void lookup(const long long* __restrict__ idx,
                                        const T* __restrict__ w, T* __restrict__ out,
                                        unsigned total, const FastDiv& per, int C, long long V,
                                        float scale, unsigned first, unsigned threads) {
-  for (unsigned i = first; i < total; i += threads) {
-    const unsigned m = per.div(i);
-    const int c = (int)(i - m * per.d) * (VEC ? 8 : 1);
-    const long long t = idx[m];
-    const bool in = t >= 0 && t < V;
-    if (c == 0) (void)MSB_OK(in, kSiteEmbeddingToken, t, V);
-    if (VEC) {
-      float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (in) load8(w + t * C + c, f);
+  constexpr int U = 4;   // in flight
+  for (unsigned i0 = first; i0 < total; i0 += U * threads) {
+    Cols<T, true> v[U];
+    T e[U];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] *= scale;
-      store8(out + (long long)m * C + c, f);
-    } else {
-      out[(long long)m * C + c] = from_f32<T>(in ? to_f32(w[t * C + c]) * scale : 0.f);
+    for (int u = 0; u < U; ++u) {
+      const unsigned i = i0 + u * threads;
+      const unsigned m = i < total ? per.div(i) : 0u;
+      const int c = (int)(i - m * per.d) * (VEC ? 8 : 1);
+      const long long t = i < total ? idx[m] : -1;
+      const bool in = t >= 0 && t < V;
+      if (c == 0 && i < total) (void)MSB_OK(in, kSiteEmbeddingToken, t, V);
+      if constexpr (VEC) {
+        v[u].load(w + (in ? t : 0) * C, c, in ? C : 0);   // zeros where not in
+      } else {
+        e[u] = in ? w[t * C + c] : from_f32<T>(0.f);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned i = i0 + u * threads;
+      if (i >= total) continue;
+      if constexpr (VEC) {   // rows lie one behind the other
+        float f[8];
+        v[u].numbers(f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] *= scale;
+        Cols<T, true>::store(out + (long long)i * 8, 0, 8, f);
+      } else {
+        out[i] = from_f32<T>(to_f32(e[u]) * scale);
+      }
     }
   }
 }
@@ -111,9 +175,11 @@ __device__ __forceinline__ void sort_tokens(const long long* __restrict__ idx, l
     auto match = [&](unsigned key, long long i) {   // the lanes with this lane's digit
       const unsigned d = (key >> shift) & ones;
       unsigned m = __ballot_sync(0xffffffffu, i < hi);
-      for (int b = 0; b < bits; ++b) {
-        const unsigned v = __ballot_sync(0xffffffffu, d >> b & 1);
-        m &= d >> b & 1 ? v : ~v;
+#pragma unroll
+      for (int b = 0; b < kDigit; ++b) {   // bits from `bits` on are 0 everywhere
+        const bool set = d >> b & 1;
+        const unsigned v = __ballot_sync(0xffffffffu, set);
+        m &= set ? v : ~v;
       }
       return m;
     };
@@ -220,47 +286,6 @@ lookup_sort_kernel(const long long* __restrict__ idx, const T* __restrict__ w,
   }
 }
 
-// Eight columns of a row as a lane holds them: packed while in flight.  VEC:
-// adjacent columns from c0 on; otherwise c0 + 32 k, for widths and addresses that
-// do not allow 16-byte accesses.
-template <typename T, bool VEC>
-struct Cols {
-  uint4 r[sizeof(T) == 4 ? 2 : 1];
-  T e[VEC ? 1 : 8];
-  __device__ __forceinline__ void load(const T* row, int c0, int C) {
-    if constexpr (VEC) {
-#pragma unroll
-      for (int k = 0; k < (int)(sizeof(T) == 4 ? 2 : 1); ++k)
-        r[k] = c0 < C ? reinterpret_cast<const uint4*>(row + c0)[k] : make_uint4(0, 0, 0, 0);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) e[k] = c0 + 32 * k < C ? row[c0 + 32 * k] : from_f32<T>(0.f);
-    }
-  }
-  __device__ __forceinline__ void numbers(float (&f)[8]) const {
-    if constexpr (!VEC) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = to_f32(e[k]);
-    } else if constexpr (sizeof(T) == 2) {
-      unpack_u4<T>(r[0], f);
-    } else {
-      const uint4 a = r[0], b = r[sizeof(T) == 4 ? 1 : 0];
-      f[0] = __uint_as_float(a.x), f[1] = __uint_as_float(a.y), f[2] = __uint_as_float(a.z),
-      f[3] = __uint_as_float(a.w), f[4] = __uint_as_float(b.x), f[5] = __uint_as_float(b.y),
-      f[6] = __uint_as_float(b.z), f[7] = __uint_as_float(b.w);
-    }
-  }
-  static __device__ __forceinline__ void store(T* row, int c0, int C, const float (&f)[8]) {
-    if constexpr (!VEC) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (c0 + 32 * k < C) row[c0 + 32 * k] = from_f32<T>(f[k]);
-    } else {
-      if (c0 < C) store8(row + c0, f);
-    }
-  }
-};
-
 // Clears the rows of a unit of `unit` table rows that no entry of the list names.
 constexpr int kUnitRows = 1024;
 template <typename T, bool VEC>
@@ -304,7 +329,7 @@ __device__ __forceinline__ void clear_unit(const uint2* __restrict__ list, long 
 }
 
 // A warp sums a chunk of CHUNK sorted entries over 256 columns.  The rows of
-// eight entries, and the gradient rows that their sums are added to, are loaded
+// four entries, and the gradient rows that their sums are added to, are loaded
 // before any is used, whatever runs they belong to: most runs are one or two
 // entries long, and run by run the loads would wait for one another.  open[j]:
 // a run begins in chunk j and goes on behind it.
@@ -513,7 +538,8 @@ void scaled_embedding_fwd(const long long* idx, const void* w, void* out, long l
         const int bits = max(2, (total_bits + passes - 1) / passes);
         unsigned R = 1;
         while (R < kMaxCluster && (long long)R * kSortThreads < n) R *= 2;
-        const unsigned gather = (grid_for(total, kSortThreads, kNumSMs * 2) + R - 1) / R * R;
+        // a block a SM in all: 64 registers a thread allow no more
+        const unsigned gather = max(R, grid_for(total, kSortThreads, kNumSMs - R) / R * R);
         uint2 *a = (uint2*)ws, *b = (uint2*)(ws + 2 * n);
         auto go = [&](auto* kernel) {
           check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
