@@ -248,7 +248,145 @@ at::Tensor scaled_embedding_bwd(const at::Tensor& dout, const at::Tensor& list, 
 
 }  // namespace
 
+// ------------------------------------------------------------- autograd
+// The operators' autograd functions.  In C++ they cost the host a third of what
+// they do in Python, which is what small calls are bound by.
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+
+bool wants_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+OptT some(const at::Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
+
+// `t` as rows of its last axis with unit column stride; copied where no view is
+at::Tensor as_rows(const at::Tensor& t) {
+  at::Tensor m = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  return m.stride(1) != 1 || (m.size(0) > 1 && m.stride(0) < m.size(1)) ? m.contiguous() : m;
+}
+
+struct TokenLogprobs : public Function<TokenLogprobs> {
+  // logprobs, then the entropy and the top log probabilities and tokens asked for
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits,
+                               const at::Tensor& tokens, double temperature, bool entropy,
+                               int64_t k, int64_t ignore_index) {
+    const at::Tensor rows = as_rows(logits), tok = tokens.contiguous();
+    auto [lp, ent, tlp, ttok, stats] = logprob_fwd(rows, tok, temperature, entropy, k, ignore_index);
+    variable_list out;
+    auto shape = tokens.sizes().vec();
+    out.push_back(lp.view(shape));
+    if (entropy) out.push_back(ent->view(shape));
+    if (k > 0) {
+      shape.push_back(k);
+      out.push_back(tlp->view(shape));
+      out.push_back(ttok->view(shape));
+    }
+    if (ctx != nullptr) {
+      ctx->set_materialize_grads(false);
+      if (k > 0) ctx->mark_non_differentiable({out.back()});
+      ctx->save_for_backward({rows, tok, k > 0 ? *ttok : at::Tensor(), stats});
+      ctx->saved_data["shape"] = logits.sizes().vec();
+      ctx->saved_data["temperature"] = temperature;
+      ctx->saved_data["entropy"] = entropy;
+      ctx->saved_data["ignore_index"] = ignore_index;
+    }
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const bool entropy = ctx->saved_data["entropy"].toBool();
+    const at::Tensor none, &gl = g[0], &ge = entropy ? g[1] : none;
+    const size_t top = entropy ? 2 : 1;
+    const at::Tensor& gt = g.size() > top ? g[top] : none;
+    at::Tensor dx;
+    if (gl.defined() || ge.defined() || gt.defined()) {
+      const auto saved = ctx->get_saved_variables();
+      dx = logprob_bwd(saved[0], saved[1], some(saved[2]), saved[3], some(gl), some(ge), some(gt),
+                       ctx->saved_data["temperature"].toDouble(),
+                       ctx->saved_data["ignore_index"].toInt())
+               .view(ctx->saved_data["shape"].toIntVector());
+    }
+    return {dx, none, none, none, none, none};
+  }
+};
+
+variable_list token_logprobs(const at::Tensor& logits, const at::Tensor& tokens,
+                             double temperature, bool entropy, int64_t k, int64_t ignore_index) {
+  if (wants_grad(logits))
+    return TokenLogprobs::apply(logits, tokens, temperature, entropy, k, ignore_index);
+  return TokenLogprobs::forward(nullptr, logits, tokens, temperature, entropy, k, ignore_index);
+}
+
+struct ScaledEmbedding : public Function<ScaledEmbedding> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& idx, const at::Tensor& weight,
+                            double scale, int64_t padding, bool sink) {
+    auto [out, list] = scaled_embedding_fwd(idx.contiguous(), weight.contiguous(), scale, padding,
+                                            ctx != nullptr);
+    if (ctx != nullptr) {
+      // the weight itself for its gradient, not for its values
+      ctx->save_for_backward({*list});
+      if (sink) ctx->saved_data["weight"] = weight;
+      ctx->saved_data["rows"] = weight.size(0);
+      ctx->saved_data["scale"] = scale;
+    }
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const at::Tensor none;
+    const at::Tensor dout = g[0].contiguous();
+    OptT sink;
+    if (ctx->saved_data.count("weight") != 0) {
+      const at::Tensor weight = ctx->saved_data["weight"].toTensor();
+      const at::Tensor& grad = weight.grad();
+      if (grad.defined() && grad.scalar_type() == weight.scalar_type() &&
+          grad.sizes() == weight.sizes() && grad.is_contiguous())
+        sink = grad;
+    }
+    const at::Tensor dw =
+        scaled_embedding_bwd(dout, ctx->get_saved_variables()[0], ctx->saved_data["rows"].toInt(),
+                             ctx->saved_data["scale"].toDouble(), sink);
+    return {none, given(sink) ? none : dw, none, none, none};
+  }
+};
+
+// `sink`: weight is a parameter, whose gradient is added to in place where it has one
+at::Tensor scaled_embedding(const at::Tensor& idx, const at::Tensor& weight, double scale,
+                            int64_t padding, bool sink) {
+  if (wants_grad(weight)) return ScaledEmbedding::apply(idx, weight, scale, padding, sink);
+  return ScaledEmbedding::forward(nullptr, idx, weight, scale, padding, sink);
+}
+
+struct SwiGLU8 : public Function<SwiGLU8> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& gu) {
+    auto [h, codes, scales] = swiglu8_fwd(gu.contiguous(), ctx != nullptr);
+    if (ctx != nullptr) ctx->save_for_backward({codes, scales});
+    return h;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    return {swiglu8_bwd(g[0].contiguous(), saved[0], saved[1])};
+  }
+};
+
+at::Tensor swiglu8(const at::Tensor& gu) {
+  return wants_grad(gu) ? SwiGLU8::apply(gu) : SwiGLU8::forward(nullptr, gu);
+}
+
+std::tuple<at::Tensor, at::Tensor> pack_rows(const at::Tensor& x) {
+  return pack8(as_rows(x.detach()));
+}
+
+}  // namespace
+
 void register_token_ops(pybind11::module_& mod) {
+  mod.def("token_logprobs", &token_logprobs);
+  mod.def("scaled_embedding", &scaled_embedding);
+  mod.def("swiglu8", &swiglu8);
+  mod.def("pack_rows", &pack_rows);
   mod.def("logprob_fwd", &logprob_fwd);
   mod.def("logprob_bwd", &logprob_bwd);
   mod.def("scaled_embedding_fwd", &scaled_embedding_fwd);

@@ -27,7 +27,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kMaxK = 32;
 constexpr int kMaxCluster = 8;
 constexpr int kGroups = 64;    // groups of threads whose maxima give a threshold, >= kMaxK
@@ -65,12 +65,6 @@ struct Vec {
                    fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
     }
   }
-  // -inf everywhere: adds nothing
-  __device__ __forceinline__ void clear() {
-    const unsigned w = sizeof(T) == 4 ? 0xff800000u
-                       : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-    r = make_uint4(w, w, w, w);
-  }
 };
 
 // (value, index) as one number: larger value first, then the lower index.
@@ -101,15 +95,21 @@ __device__ __forceinline__ float reference(float m, float c) {   // of -inf: 0
 // 0 * z a number
 constexpr float kLowZ = -200.f;
 
-// a thread's running maximum, its reference, and the sums relative to it
+// A thread's maximum, and its sums relative to a reference that trails it: only
+// a value more than 2^kSlack above moves it.  Some lane of a warp finds a new
+// maximum in most vectors, so following it exactly would rescale in most.
+constexpr float kSlack = 16.f;
 struct Sums {
-  float m = -INFINITY, ref = 0.f, s = 0.f, t = 0.f;
-  // to a reference above; from that of nothing yet (0) to any
-  __device__ __forceinline__ void rebase(float to) {
+  float m = -INFINITY, ref = -1e37f, s = 0.f, t = 0.f;
+  __device__ __forceinline__ void rebase(float to) {   // to a reference above
     const float d = fminf(fmaxf(ref - to, kLowZ), 0.f), f = ex2_approx(d);
     t = f * (t + s * d);
     s *= f;
     ref = to;
+  }
+  __device__ __forceinline__ void see(float v, float c) {
+    m = fmaxf(m, v);
+    if (fmaf(v, c, -ref) > kSlack) rebase(reference(v, c));
   }
 };
 
@@ -124,11 +124,7 @@ __device__ __forceinline__ void add_z(float z, float& s, float& t) {
 template <typename T, bool ENT>
 __device__ __forceinline__ void add_vec(Sums& a, const Vec<T>& v, float c) {
   constexpr int N = Vec<T>::N;
-  const float m = v.max();
-  if (m > a.m) {
-    a.rebase(reference(m, c));
-    a.m = m;
-  }
+  a.see(v.max(), c);
   float x[N], s1 = 0.f, t1 = 0.f;
   v.unpack(x);
 #pragma unroll
@@ -142,10 +138,7 @@ __device__ __forceinline__ void add_vec(Sums& a, const Vec<T>& v, float c) {
 
 template <bool ENT>
 __device__ __forceinline__ void add_one(Sums& a, float x, float c) {
-  if (x > a.m) {
-    a.rebase(reference(x, c));
-    a.m = x;
-  }
+  a.see(x, c);
   add_z<ENT>(fmaf(x, c, -a.ref), a.s, a.t);
 }
 
@@ -193,13 +186,15 @@ __device__ __forceinline__ float block_reduce(float v, float* buf, F&& f) {
 }
 
 // What a block knows of its part of the row, read by the cluster's first block.
-struct alignas(8) Shared {
+struct Common {
+  float ms[3];                         // maximum, s, t
+  float buf[3][kThreads / 32];
+};
+struct Top {
   unsigned long long best[kMaxK];      // its alternatives, best first; 0: none
   unsigned long long cand[kCand];
   unsigned long long equal[kEqual];
   unsigned long long round[kThreads / 32];
-  float ms[3];                         // maximum, s, t
-  float buf[3][kThreads / 32];
   float thread_max[kThreads];
   unsigned group[kGroups];
   unsigned short winner[kThreads];
@@ -226,7 +221,7 @@ __device__ __forceinline__ void rank_keys(const unsigned long long* keys, int n,
 // Values equal to it are taken in index order: collected too or, where a row
 // has very many (a mask), found by a scan from the front.
 template <typename T>
-__device__ void top_of_part(const Part<T>& p, float my_max, int k, Shared& sh) {
+__device__ void top_of_part(const Part<T>& p, float my_max, int k, Top& sh) {
   constexpr int N = Vec<T>::N;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   sh.thread_max[tid] = my_max;
@@ -349,7 +344,8 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
                    float* __restrict__ top_logp, long long* __restrict__ top_tok,
                    float* __restrict__ stats) {
   ::msb::pdl_begin();
-  __shared__ Shared sh;
+  __shared__ Common sh;
+  __shared__ std::conditional_t<TOP, Top, int> top;
   cg::cluster_group cluster = cg::this_cluster();
   const unsigned R = cluster.num_blocks(), q = cluster.block_rank();
   const long long r = blockIdx.x / R;
@@ -376,15 +372,11 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   for (int v = p.v0 + tid; v < p.v1; v += U * kThreads) {
     Vec<T> x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (v + u * kThreads < p.v1) {
-        x[u].r = p.mid[v + u * kThreads];
-      } else {
-        x[u].clear();
-      }
-    }
+    for (int u = 0; u < U; ++u)
+      if (v + u * kThreads < p.v1) x[u].r = p.mid[v + u * kThreads];
 #pragma unroll
-    for (int u = 0; u < U; ++u) add_vec<T, ENT>(a, x[u], c);
+    for (int u = 0; u < U; ++u)
+      if (v + u * kThreads < p.v1) add_vec<T, ENT>(a, x[u], c);
   }
   if (tid < p.loose()) add_one<ENT>(a, to_f32(row[p.loose_at(tid)]), c);
   const float my_max = a.m;
@@ -410,7 +402,7 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   }
   float s = block_reduce(a.s, sh.buf[1], sum);
   float tt = ENT ? block_reduce(a.t, sh.buf[2], sum) : 0.f;
-  if (TOP) top_of_part(p, my_max, k, sh);
+  if constexpr (TOP) top_of_part(p, my_max, k, top);
   if (R > 1) {
     if (tid == 0) {
       sh.ms[1] = s;
@@ -424,17 +416,17 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
         s += o[1];
         tt += o[2];
       }
-      if (TOP) {
+      if constexpr (TOP) {
         for (int i = tid; i < (int)R * k; i += kThreads)
-          sh.cand[i] = cluster.map_shared_rank(sh.best, i / k)[i % k];
+          top.cand[i] = cluster.map_shared_rank(top.best, i / k)[i % k];
       }
     }
     cluster.sync();   // the other blocks' shared memory has been read
     if (q != 0) return;
-    if (TOP) {
-      if (tid < k) sh.best[tid] = 0;
+    if constexpr (TOP) {
+      if (tid < k) top.best[tid] = 0;
       __syncthreads();
-      rank_keys(sh.cand, (int)R * k, sh.best, k);
+      rank_keys(top.cand, (int)R * k, top.best, k);
       __syncthreads();
     }
   }
@@ -458,11 +450,13 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
     stats[r * 3 + 1] = s;
     stats[r * 3 + 2] = tt;
   }
-  if (TOP && tid < k) {
-    const unsigned long long b = sh.best[tid];   // 0: a row of NaN
-    const int i = b == 0 ? 0 : key_index(b);
-    top_tok[r * k + tid] = i;
-    top_logp[r * k + tid] = value(to_f32(row[i]));
+  if constexpr (TOP) {
+    if (tid < k) {
+      const unsigned long long b = top.best[tid];   // 0: a row of NaN
+      const int i = b == 0 ? 0 : key_index(b);
+      top_tok[r * k + tid] = i;
+      top_logp[r * k + tid] = value(to_f32(row[i]));
+    }
   }
 }
 
@@ -577,11 +571,14 @@ logprob_bwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   }
 }
 
-// Blocks a row: twice the SMs' number in all where rows are few, as long as a
-// block keeps half of its threads busy with a vector.
-unsigned blocks_a_row(long long M, int V, int per_vec) {
+// Blocks a row: `a_sm` a SM in all where rows are few, as long as a block has two
+// vectors a thread.  The forward's blocks wait for one another, and more than it
+// takes to fill the GPU cost more than they bring (2048 x 128256 bf16: 109 us
+// with one, 131 with four); the backward's are independent, and even out the
+// last rows (182 us with one, 168 with four).
+unsigned blocks_a_row(long long M, int V, int per_vec, int a_sm) {
   unsigned R = 1;
-  while (R < kMaxCluster && M * R < 2 * kNumSMs && V / (int)(2 * R) >= per_vec * kThreads / 2) R *= 2;
+  while (R < kMaxCluster && M * R < a_sm * kNumSMs && V / (int)(2 * R) >= per_vec * kThreads) R *= 2;
   return R;
 }
 
@@ -594,7 +591,7 @@ void logprob_fwd(const void* logits, long long ld, const long long* tok, long lo
   const float c = (float)(1.4426950408889634 / (double)temperature);
   const float inv_t = (float)(1.0 / (double)temperature);
   MSB_DISPATCH_FLOAT(dtype, T, {
-    const unsigned R = blocks_a_row(M, V, Vec<T>::N);
+    const unsigned R = blocks_a_row(M, V, Vec<T>::N, 4);
     auto go = [&](auto* kernel) {
       launch_cluster(R, kernel, (unsigned)M * R, kThreads, 0, st, (const T*)logits, ld, tok, V, c,
                      inv_t, ignore_index, k, logp, entropy, top_logp, top_tok, stats);
@@ -616,7 +613,7 @@ void logprob_bwd(const void* logits, long long ld, const long long* tok, long lo
   const float c = (float)(1.4426950408889634 / (double)temperature);
   const float inv_t = (float)(1.0 / (double)temperature);
   MSB_DISPATCH_FLOAT(dtype, T, {
-    const unsigned R = blocks_a_row(M, V, Vec<T>::N);
+    const unsigned R = blocks_a_row(M, V, Vec<T>::N, 32);
     auto go = [&](auto* kernel) {
       launch(kernel, (unsigned)M * R, kThreads, 0, st, (const T*)logits, ld, tok, M, V, c, inv_t,
              ignore_index, k, top_tok, stats, g_logp, g_ent, g_top, (T*)dx, ld_dx, R);

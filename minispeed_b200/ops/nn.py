@@ -31,7 +31,6 @@ from __future__ import annotations
 
 import math
 from contextlib import contextmanager
-from dataclasses import dataclass
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -426,32 +425,17 @@ class _SwiGLU(torch.autograd.Function):
         return dgu
 
 
-class _SwiGLU8(torch.autograd.Function):
-    """SwiGLU that saves its input packed: the forward kernel writes the codes
-    in the pass that computes ``h``, the backward kernel reads them in place of
-    the input."""
-
+class _SwiGLU8CPU(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gu):
-        ctx.set_materialize_grads(False)
-        if gu.is_cuda:
-            h, codes, scales = _C().swiglu8_fwd(gu, True)
-        else:
-            F_ = gu.shape[-1] // 2
-            codes, scales = _pack8_torch(gu.reshape(-1, F_))
-            h = _swiglu_torch(gu)
-        ctx.save_for_backward(codes, scales)
-        return h
+        F_ = gu.shape[-1] // 2
+        ctx.save_for_backward(*_pack8_torch(gu.reshape(-1, F_)))
+        return _swiglu_torch(gu)
 
     @staticmethod
     def backward(ctx, dh):
-        if dh is None:
-            return None
-        codes, scales = ctx.saved_tensors
-        if dh.is_cuda:
-            return _C().swiglu8_bwd(dh.contiguous(), codes, scales)
         F_ = dh.shape[-1]
-        g, u = _unpack8_torch(codes, scales, F_).view(-1, 2, F_).unbind(1)
+        g, u = _unpack8_torch(*ctx.saved_tensors, F_).view(-1, 2, F_).unbind(1)
         d = dh.reshape(-1, F_).float()
         s = torch.sigmoid(g)
         dgu = torch.cat([d * u * s * (1 + g * (1 - s)), d * g * s], -1)
@@ -481,11 +465,9 @@ def swiglu(gu: torch.Tensor, save_bits: Optional[int] = None) -> torch.Tensor:
         _check_packable(gu)
         if gu.shape[-1] % 2:
             raise ValueError(f"swiglu: the last axis holds [gate | up], got width {gu.shape[-1]}")
-        if gu.numel() and torch.is_grad_enabled() and gu.requires_grad:
-            return _SwiGLU8.apply(gu.contiguous())
-        if gu.numel() and gu.is_cuda:
-            return _C().swiglu8_fwd(gu.contiguous(), False)[0]
-        return _swiglu_torch(gu)
+        if not gu.numel():
+            return _swiglu_torch(gu)
+        return _C().swiglu8(gu) if gu.is_cuda else _SwiGLU8CPU.apply(gu)
     if gu.is_cuda:
         return _SwiGLU.apply(gu.contiguous())
     return _swiglu_torch(gu)
@@ -520,16 +502,17 @@ def _unpack8_torch(codes: torch.Tensor, scales: torch.Tensor, width: int) -> tor
     return torch.where(b == 255, float("nan"), f).flatten(-2)[..., :width]
 
 
-@dataclass(frozen=True)
 class PackedActivation:
-    """A tensor held in 8 bits: one signed byte a value and one byte, the
-    exponent of a power-of-two scale, for every 32 values of the last axis (the
-    last block of a row may be short)."""
+    """A tensor held in 8 bits: one signed byte a value (``codes``, int8
+    [rows, 32 * blocks]) and one byte, the exponent of a power-of-two scale, for
+    every 32 values of the last axis (``scales``, uint8 [rows, blocks]; the last
+    block of a row may be short); and its ``shape`` and ``dtype``."""
 
-    codes: torch.Tensor        # int8 [rows, 32 * blocks]
-    scales: torch.Tensor       # uint8 [rows, blocks]
-    shape: torch.Size
-    dtype: torch.dtype
+    __slots__ = ("codes", "scales", "shape", "dtype")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: torch.Size,
+                 dtype: torch.dtype):
+        self.codes, self.scales, self.shape, self.dtype = codes, scales, shape, dtype
 
     def unpack(self) -> torch.Tensor:
         """The tensor again, contiguous, in its own type.  Values are off by at
@@ -554,12 +537,11 @@ def pack_activation(x: torch.Tensor) -> PackedActivation:
     :meth:`PackedActivation.unpack` brings it back.  No gradient flows through
     the pair: it is for what a backward pass keeps."""
     _check_packable(x)
-    x = x.detach()
     if not x.numel():
         empty = x.new_empty((0, 0), dtype=torch.uint8)
         return PackedActivation(empty.view(torch.int8), empty, x.shape, x.dtype)
-    x2 = as_matrix(x, x.shape[-1])
-    codes, scales = _C().pack8(x2) if x.is_cuda else _pack8_torch(x2)
+    codes, scales = _C().pack_rows(x) if x.is_cuda else \
+        _pack8_torch(as_matrix(x.detach(), x.shape[-1]))
     return PackedActivation(codes, scales, x.shape, x.dtype)
 
 
@@ -648,32 +630,6 @@ class TokenLogprobs(NamedTuple):
     top_tokens: Optional[torch.Tensor]     # int64 [..., k]
 
 
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, temperature, entropy, top_k, ignore_index):
-        ctx.set_materialize_grads(False)
-        l2 = as_matrix(logits, logits.shape[-1])
-        t = tokens.reshape(-1).contiguous()
-        lp, ent, top_lp, top, stats = _C().logprob_fwd(l2, t, temperature, entropy, top_k,
-                                                       ignore_index)
-        ctx.save_for_backward(l2, t, top, stats)
-        ctx.shape = logits.shape
-        ctx.args = (temperature, ignore_index)
-        shape = tokens.shape
-        if top is not None:
-            top_lp, top = top_lp.view(*shape, top_k), top.view(*shape, top_k)
-            ctx.mark_non_differentiable(top)
-        return lp.view(shape), None if ent is None else ent.view(shape), top_lp, top
-
-    @staticmethod
-    def backward(ctx, g_lp, g_ent, g_top, _):
-        if g_lp is None and g_ent is None and g_top is None:
-            return (None,) * 6
-        l2, t, top, stats = ctx.saved_tensors
-        dx = _C().logprob_bwd(l2, t, top, stats, g_lp, g_ent, g_top, *ctx.args)
-        return (dx.view(ctx.shape),) + (None,) * 5
-
-
 def _token_logprobs_torch(logits, tokens, temperature, entropy, top_k, ignore_index):
     """The same in PyTorch operations."""
     keep = tokens != ignore_index
@@ -746,9 +702,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
         raise ValueError(f"token_logprobs: temperature must be between 1e-30 and 1e30, got "
                          f"{temperature}")
     args = (float(temperature), bool(entropy), int(top_k), int(ignore_index))
-    if logits.is_cuda and logits.numel():
-        return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, *args))
-    return TokenLogprobs(*_token_logprobs_torch(logits, tokens, *args))
+    if not (logits.is_cuda and logits.numel()):
+        return TokenLogprobs(*_token_logprobs_torch(logits, tokens, *args))
+    r = _C().token_logprobs(logits, tokens, *args)
+    return TokenLogprobs(r[0], r[1] if entropy else None, *(r[-2:] if top_k else (None, None)))
 
 
 # ------------------------------------------------------------ embedding
@@ -816,32 +773,22 @@ def embedding(idx: torch.Tensor, wte: torch.Tensor, wpe: Optional[torch.Tensor] 
     return x
 
 
-class _ScaledEmbedding(torch.autograd.Function):
+class _ScaledEmbeddingCPU(torch.autograd.Function):
     @staticmethod
     def forward(ctx, idx, weight, scale, padding):
-        if weight.is_cuda:
-            # what backward needs of the tokens is their sorted list
-            out, kept = _C().scaled_embedding_fwd(idx.contiguous(), weight.contiguous(), scale,
-                                                  padding, ctx.needs_input_grad[1])
-        else:
-            out, kept = (F.embedding(idx, weight).float() * scale).to(weight.dtype), idx
-        ctx.save_for_backward(kept)
+        ctx.save_for_backward(idx)
         ctx.weight = weight
-        ctx.args = (weight.shape[0], padding, scale)
-        return out
+        ctx.args = (padding, scale)
+        return (F.embedding(idx, weight).float() * scale).to(weight.dtype)
 
     @staticmethod
     def backward(ctx, dout):
-        (kept,) = ctx.saved_tensors
-        V, padding, scale = ctx.args
-        sink = grad_sink(ctx.weight)
-        if dout.is_cuda:
-            dw = _C().scaled_embedding_bwd(dout.contiguous(), kept, V, scale, sink)
-            return None, None if sink is not None else dw, None, None
-        idx = kept.reshape(-1)
+        (idx,) = ctx.saved_tensors
+        padding, scale = ctx.args
+        idx = idx.reshape(-1)
         rows = dout.reshape(idx.numel(), -1).float() * scale
         rows = torch.where((idx == padding)[:, None], 0.0, rows)
-        dw = torch.zeros(V, dout.shape[-1]).index_add_(0, idx, rows)
+        dw = torch.zeros(ctx.weight.shape).index_add_(0, idx, rows)
         return None, dw.to(dout.dtype), None, None
 
 
@@ -875,7 +822,9 @@ def scaled_embedding(idx: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
             raise ValueError(f"scaled_embedding: padding_idx {padding_idx} outside a table of "
                              f"{V} rows")
         padding = padding_idx % V
-    return _ScaledEmbedding.apply(idx, weight, float(scale), padding)
+    if not weight.is_cuda:
+        return _ScaledEmbeddingCPU.apply(idx, weight, float(scale), padding)
+    return _C().scaled_embedding(idx, weight, scale, padding, isinstance(weight, torch.nn.Parameter))
 
 
 # ------------------------------------------------------------------ rope
