@@ -33,7 +33,7 @@ constexpr int kMaxCluster = 8;
 constexpr int kGroups = 64;    // groups of threads whose maxima give a threshold, >= kMaxK
 constexpr int kCand = 1024;    // candidates kept above the threshold, and
 constexpr int kEqual = 512;    // at it
-static_assert(kMaxK <= kGroups && kMaxK + kEqual <= kCand && kMaxCluster * kMaxK <= kCand, "");
+static_assert(kGroups * 4 == kThreads && kMaxK <= kGroups && kMaxK + kEqual <= kCand && kMaxCluster * kMaxK <= kCand, "");
 
 // 16 bytes of logits
 template <typename T>
@@ -72,6 +72,9 @@ struct Vec {
 __device__ __forceinline__ unsigned order_of(float v) {
   const int b = __float_as_int(v + 0.f);  // -0 counts as 0
   return b < 0 ? ~(unsigned)b : (unsigned)b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(unsigned u) {
+  return __int_as_float((int)(u & 0x80000000u ? u & 0x7fffffffu : ~u));
 }
 __device__ __forceinline__ unsigned long long key_of(float v, int i) {
   return v != v ? 0ull : ((unsigned long long)order_of(v) << 32) | (0xffffffffu - (unsigned)i);
@@ -173,13 +176,16 @@ struct Part {
   }
 };
 
+// A reduction over the block in two halves, so that several share one barrier.
 template <typename F>
-__device__ __forceinline__ float block_reduce(float v, float* buf, F&& f) {
+__device__ __forceinline__ void reduce_warps(float v, float* buf, F&& f) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
   if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = buf[threadIdx.x & (kThreads / 32 - 1)];
+}
+template <typename F>
+__device__ __forceinline__ float reduce_block(const float* buf, F&& f) {   // after a barrier
+  float v = buf[threadIdx.x & (kThreads / 32 - 1)];
 #pragma unroll
   for (int o = kThreads / 64; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
@@ -190,12 +196,11 @@ struct Common {
   float ms[3];                         // maximum, s, t
   float buf[3][kThreads / 32];
 };
-struct Top {
+struct alignas(16) Top {
   unsigned long long best[kMaxK];      // its alternatives, best first; 0: none
   unsigned long long cand[kCand];
   unsigned long long equal[kEqual];
   unsigned long long round[kThreads / 32];
-  float thread_max[kThreads];
   unsigned group[kGroups];
   unsigned short winner[kThreads];
   float threshold;
@@ -208,44 +213,55 @@ __device__ __forceinline__ void rank_keys(const unsigned long long* keys, int n,
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const unsigned long long mine = keys[i];
     if (mine == 0) continue;
-    int r = 0;
-    for (int j = 0; j < n; ++j) r += keys[j] > mine;
+    int r = 0, j = 0;
+#pragma unroll 4
+    for (; j + 2 <= n; j += 2) {
+      const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(keys + j);
+      r += (two.x > mine) + (two.y > mine);
+    }
+    if (j < n) r += keys[j] > mine;
     if (r < k) out[r] = mine;
   }
 }
 
 // The block's k best values.  Every thread has the maximum of its values; the
-// k-th largest of 64 group maxima is a threshold that at least k values reach
-// and few exceed.  Only the values of the threads whose maximum reaches it are
-// read again (from L2), the ones above the threshold collected and ranked.
-// Values equal to it are taken in index order: collected too or, where a row
-// has very many (a mask), found by a scan from the front.
+// k-th largest of 64 maxima of four threads each is a threshold that at least k
+// values reach and few exceed.  Only the values of the threads whose maximum
+// reaches it are read again (from L2), the ones above the threshold collected
+// and ranked.  Values equal to it are taken in index order: collected too or,
+// where a row has very many (a mask), found by a scan from the front.
+//
+// Three steps with a barrier after each of the first two, which the kernel
+// shares with its sums.
+__device__ __forceinline__ void top_groups(float my_max, int k, Top& sh) {
+  constexpr int A_WARP = kGroups / (kThreads / 32);
+  const int tid = threadIdx.x, lane = tid & 31;
+  float m = my_max;
+#pragma unroll
+  for (int o = A_WARP; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane < A_WARP) sh.group[(tid >> 5) * A_WARP + lane] = order_of(m);
+  if (tid < k) sh.best[tid] = 0;
+  if (tid == 0) sh.winners = sh.above = sh.at = 0;
+}
+__device__ __forceinline__ void top_threshold(int k, Top& sh) {
+  const int tid = threadIdx.x;
+  if (tid >= kGroups) return;
+  const unsigned mine = sh.group[tid];
+  int r = 0;
+#pragma unroll 4
+  for (int j = 0; j < kGroups; j += 4) {
+    const uint4 o = *reinterpret_cast<const uint4*>(sh.group + j);
+    r += o.x > mine || (o.x == mine && j < tid);
+    r += o.y > mine || (o.y == mine && j + 1 < tid);
+    r += o.z > mine || (o.z == mine && j + 2 < tid);
+    r += o.w > mine || (o.w == mine && j + 3 < tid);
+  }
+  if (r == k - 1) sh.threshold = value_of(mine);
+}
 template <typename T>
 __device__ void top_of_part(const Part<T>& p, float my_max, int k, Top& sh) {
   constexpr int N = Vec<T>::N;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  sh.thread_max[tid] = my_max;
-  if (tid < k) sh.best[tid] = 0;
-  if (tid == 0) sh.winners = sh.above = sh.at = 0;
-  __syncthreads();
-  float gmax = -INFINITY;
-  if (tid < kGroups) {
-#pragma unroll
-    for (int j = 0; j < kThreads / kGroups; ++j) gmax = fmaxf(gmax, sh.thread_max[tid + kGroups * j]);
-    sh.group[tid] = order_of(gmax);
-  }
-  __syncthreads();
-  if (tid < kGroups) {
-    const unsigned mine = sh.group[tid];
-    int r = 0;
-#pragma unroll 16
-    for (int j = 0; j < kGroups; ++j) {
-      const unsigned o = sh.group[j];
-      r += o > mine || (o == mine && j < tid);
-    }
-    if (r == k - 1) sh.threshold = gmax;
-  }
-  __syncthreads();
   const float thr = sh.threshold;
   if (my_max >= thr) sh.winner[atomicAdd(&sh.winners, 1)] = (unsigned short)tid;
   __syncthreads();
@@ -259,16 +275,24 @@ __device__ void top_of_part(const Part<T>& p, float my_max, int k, Top& sh) {
     }
   };
   const int each = (p.v1 - p.v0 + kThreads - 1) / kThreads, items = sh.winners * each;
-  for (int i = tid; i < items; i += kThreads) {
-    const int w = i / each, v = p.v0 + sh.winner[w] + (i - w * each) * kThreads;
-    if (v >= p.v1) continue;
-    Vec<T> x;
-    x.r = p.mid[v];
-    if (!(x.max() >= thr)) continue;
-    float f[N];
-    x.unpack(f);
+  constexpr int U = 4;   // in flight
+  for (int i0 = tid; i0 < items; i0 += U * kThreads) {
+    Vec<T> x[U];
+    int v[U];
 #pragma unroll
-    for (int j = 0; j < N; ++j) take(f[j], p.at(v) + j);
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kThreads, w = i / each;
+      v[u] = i < items ? p.v0 + sh.winner[w] + (i - w * each) * kThreads : p.v1;
+      if (v[u] < p.v1) x[u].r = p.mid[v[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (v[u] >= p.v1 || !(x[u].max() >= thr)) continue;
+      float f[N];
+      x[u].unpack(f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) take(f[j], p.at(v[u]) + j);
+    }
   }
   for (int i = tid; i < p.loose(); i += kThreads) {
     const int at = p.loose_at(i);
@@ -337,7 +361,7 @@ __device__ void top_of_part(const Part<T>& p, float my_max, int k, Top& sh) {
 
 // A cluster a row (of one block where there are rows enough).
 template <typename T, bool ENT, bool TOP>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 6)
 logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* __restrict__ tok,
                    int V, float c, float inv_t, long long ignore_index, int k,
                    float* __restrict__ logp, float* __restrict__ entropy,
@@ -383,14 +407,17 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
 
   auto larger = [](float x, float y) { return fmaxf(x, y); };
   auto sum = [](float x, float y) { return x + y; };
-  float m = block_reduce(my_max, sh.buf[0], larger);
+  reduce_warps(my_max, sh.buf[0], larger);
+  if constexpr (TOP) top_groups(my_max, k, top);
+  __syncthreads();
+  float m = reduce_block(sh.buf[0], larger);
   if (R > 1) {   // the row's maximum
     if (tid == 0) sh.ms[0] = m;
     cluster.sync();
     for (unsigned b = 0; b < R; ++b) m = fmaxf(m, cluster.map_shared_rank(sh.ms, b)[0]);
   }
   const bool wide = is_wide(m, c);
-  float ref = reference(m, c);
+  const float ref = reference(m, c);
   if (wide && m != INFINITY) {   // once more, with differences
     a.s = a.t = 0.f;
     for (int i = p.at(p.v0) + tid; i < p.at(p.v1); i += kThreads)
@@ -400,8 +427,11 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   } else {
     a.rebase(ref);
   }
-  float s = block_reduce(a.s, sh.buf[1], sum);
-  float tt = ENT ? block_reduce(a.t, sh.buf[2], sum) : 0.f;
+  reduce_warps(a.s, sh.buf[1], sum);
+  if (ENT) reduce_warps(a.t, sh.buf[2], sum);
+  if constexpr (TOP) top_threshold(k, top);
+  __syncthreads();
+  float s = reduce_block(sh.buf[1], sum), tt = ENT ? reduce_block(sh.buf[2], sum) : 0.f;
   if constexpr (TOP) top_of_part(p, my_max, k, top);
   if (R > 1) {
     if (tid == 0) {
@@ -453,9 +483,8 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   if constexpr (TOP) {
     if (tid < k) {
       const unsigned long long b = top.best[tid];   // 0: a row of NaN
-      const int i = b == 0 ? 0 : key_index(b);
-      top_tok[r * k + tid] = i;
-      top_logp[r * k + tid] = value(to_f32(row[i]));
+      top_tok[r * k + tid] = b == 0 ? 0 : key_index(b);
+      top_logp[r * k + tid] = b == 0 ? NAN : value(value_of((unsigned)(b >> 32)));
     }
   }
 }
@@ -591,7 +620,7 @@ void logprob_fwd(const void* logits, long long ld, const long long* tok, long lo
   const float c = (float)(1.4426950408889634 / (double)temperature);
   const float inv_t = (float)(1.0 / (double)temperature);
   MSB_DISPATCH_FLOAT(dtype, T, {
-    const unsigned R = blocks_a_row(M, V, Vec<T>::N, 4);
+    const unsigned R = blocks_a_row(M, V, Vec<T>::N, 2);
     auto go = [&](auto* kernel) {
       launch_cluster(R, kernel, (unsigned)M * R, kThreads, 0, st, (const T*)logits, ld, tok, V, c,
                      inv_t, ignore_index, k, logp, entropy, top_logp, top_tok, stats);
