@@ -77,16 +77,20 @@ std::tuple<at::Tensor, at::Tensor> pack8(const at::Tensor& x) {
   return out;
 }
 
-// dtype: an msb::DType code
-at::Tensor unpack8(const at::Tensor& codes, const at::Tensor& scales, int64_t width, int64_t code) {
+// a new tensor of `shape`; dtype: an msb::DType code
+at::Tensor unpack8(const at::Tensor& codes, const at::Tensor& scales, at::IntArrayRef shape,
+                   int64_t code) {
   TORCH_CHECK(code == msb::kF32 || code == msb::kF16 || code == msb::kBF16, "dtype code");
   const at::ScalarType dtype =
       code == msb::kF32 ? at::kFloat : code == msb::kF16 ? at::kHalf : at::kBFloat16;
-  TORCH_CHECK(codes.dim() == 2 && width > 0, "codes: int8 [rows, 32 * blocks]");
-  check_packed(codes, scales, codes.size(0), width);
+  TORCH_CHECK(codes.dim() == 2 && !shape.empty() && shape.back() > 0,
+              "codes: int8 [rows, 32 * blocks] of a shape");
+  const int64_t rows = codes.size(0), width = shape.back();
+  check_packed(codes, scales, rows, width);
   c10::cuda::CUDAGuard g(codes.device());
-  at::Tensor x = at::empty({codes.size(0), width}, codes.options().dtype(dtype));
-  msb::unpack8(codes_of(codes), bytes(scales), x.data_ptr(), x.size(0), (int)width, dtype_code(x),
+  at::Tensor x = at::empty(shape, codes.options().dtype(dtype));
+  TORCH_CHECK(x.numel() == rows * width && width < (1LL << 31) - 1024, "shape of another tensor");
+  msb::unpack8(codes_of(codes), bytes(scales), x.data_ptr(), rows, (int)width, (int)code,
                stream_of(codes));
   return x;
 }
@@ -377,7 +381,7 @@ at::Tensor swiglu8(const at::Tensor& gu) {
 }
 
 std::tuple<at::Tensor, at::Tensor> pack_rows(const at::Tensor& x) {
-  return pack8(as_rows(x.detach()));
+  return pack8(as_rows(x.requires_grad() ? x.detach() : x));
 }
 
 }  // namespace

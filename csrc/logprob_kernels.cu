@@ -103,11 +103,12 @@ constexpr float kLowZ = -200.f;
 // maximum in most vectors, so following it exactly would rescale in most.
 constexpr float kSlack = 16.f;
 struct Sums {
-  float m = -INFINITY, ref = -1e37f, s = 0.f, t = 0.f;
+  float m = -INFINITY, ref = -1e37f;
+  float2 s = {0.f, 0.f}, t = {0.f, 0.f};   // of even and odd values
   __device__ __forceinline__ void rebase(float to) {   // to a reference above
     const float d = fminf(fmaxf(ref - to, kLowZ), 0.f), f = ex2_approx(d);
-    t = f * (t + s * d);
-    s *= f;
+    t = make_float2(f * fmaf(s.x, d, t.x), f * fmaf(s.y, d, t.y));
+    s = make_float2(s.x * f, s.y * f);
     ref = to;
   }
   __device__ __forceinline__ void see(float v, float c) {
@@ -117,32 +118,28 @@ struct Sums {
 };
 
 template <bool ENT>
-__device__ __forceinline__ void add_z(float z, float& s, float& t) {
-  if (ENT) z = max_nan(z, kLowZ);
-  const float e = ex2_approx(z);
-  s += e;
-  if (ENT) t = fmaf(e, z, t);
+__device__ __forceinline__ void add_z(Sums& a, float2 z) {
+  if (ENT) z = make_float2(max_nan(z.x, kLowZ), max_nan(z.y, kLowZ));
+  const float2 e = make_float2(ex2_approx(z.x), ex2_approx(z.y));
+  a.s = add2(a.s, e);
+  if (ENT) a.t = fma2(e, z, a.t);
 }
 
 template <typename T, bool ENT>
 __device__ __forceinline__ void add_vec(Sums& a, const Vec<T>& v, float c) {
   constexpr int N = Vec<T>::N;
   a.see(v.max(), c);
-  float x[N], s1 = 0.f, t1 = 0.f;
+  float x[N];
   v.unpack(x);
+  const float2 c2 = make_float2(c, c), r2 = make_float2(-a.ref, -a.ref);
 #pragma unroll
-  for (int k = 0; k < N; k += 2) {
-    add_z<ENT>(fmaf(x[k], c, -a.ref), a.s, a.t);
-    add_z<ENT>(fmaf(x[k + 1], c, -a.ref), s1, t1);
-  }
-  a.s += s1;
-  a.t += t1;
+  for (int k = 0; k < N; k += 2) add_z<ENT>(a, fma2(make_float2(x[k], x[k + 1]), c2, r2));
 }
 
 template <bool ENT>
 __device__ __forceinline__ void add_one(Sums& a, float x, float c) {
   a.see(x, c);
-  add_z<ENT>(fmaf(x, c, -a.ref), a.s, a.t);
+  add_z<ENT>(a, make_float2(fmaf(x, c, -a.ref), -INFINITY));
 }
 
 // The part of a row that a block of the cluster reads: vectors [v0, v1) of the
@@ -419,16 +416,16 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   const bool wide = is_wide(m, c);
   const float ref = reference(m, c);
   if (wide && m != INFINITY) {   // once more, with differences
-    a.s = a.t = 0.f;
+    a.s = a.t = make_float2(0.f, 0.f);
     for (int i = p.at(p.v0) + tid; i < p.at(p.v1); i += kThreads)
-      add_z<ENT>((to_f32(row[i]) - m) * c, a.s, a.t);
+      add_z<ENT>(a, make_float2((to_f32(row[i]) - m) * c, -INFINITY));
     for (int i = tid; i < p.loose(); i += kThreads)
-      add_z<ENT>((to_f32(row[p.loose_at(i)]) - m) * c, a.s, a.t);
+      add_z<ENT>(a, make_float2((to_f32(row[p.loose_at(i)]) - m) * c, -INFINITY));
   } else {
     a.rebase(ref);
   }
-  reduce_warps(a.s, sh.buf[1], sum);
-  if (ENT) reduce_warps(a.t, sh.buf[2], sum);
+  reduce_warps(a.s.x + a.s.y, sh.buf[1], sum);
+  if (ENT) reduce_warps(a.t.x + a.t.y, sh.buf[2], sum);
   if constexpr (TOP) top_threshold(k, top);
   __syncthreads();
   float s = reduce_block(sh.buf[1], sum), tt = ENT ? reduce_block(sh.buf[2], sum) : 0.f;

@@ -36,6 +36,24 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
+// two fp32 operations in one instruction
+__device__ __forceinline__ unsigned long long bits_of(float2 v) {
+  return (unsigned long long)__float_as_uint(v.y) << 32 | __float_as_uint(v.x);
+}
+__device__ __forceinline__ float2 pair_of(unsigned long long b) {
+  return make_float2(__uint_as_float((unsigned)b), __uint_as_float((unsigned)(b >> 32)));
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits_of(a)), "l"(bits_of(b)), "l"(bits_of(c)));
+  return pair_of(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits_of(a)), "l"(bits_of(b)));
+  return pair_of(d);
+}
+
 // 8-element accesses: one 16-byte transaction when the address allows it,
 // element-wise otherwise.  Parameters are views into a flat arena at
 // arbitrary element offsets, so weights and biases need not be aligned.

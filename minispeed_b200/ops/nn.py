@@ -519,13 +519,12 @@ class PackedActivation:
         most half a step of their block's scale, 2^-7 of its largest magnitude
         (a whole step for values that round to 128 steps); a block that held an
         infinity or a NaN is all NaN."""
-        if not self.scales.numel():
+        if 0 in self.shape:
             return torch.empty(self.shape, dtype=self.dtype, device=self.codes.device)
         if self.codes.is_cuda:
-            x = _C().unpack8(self.codes, self.scales, self.shape[-1], _DTYPE_CODES[self.dtype])
-        else:
-            x = _unpack8_torch(self.codes, self.scales, self.shape[-1]).to(self.dtype)
-        return x.view(self.shape)
+            return _C().unpack8(self.codes, self.scales, self.shape, _DTYPE_CODES[self.dtype])
+        x = _unpack8_torch(self.codes, self.scales, self.shape[-1])
+        return x.to(self.dtype).view(self.shape)
 
     @property
     def nbytes(self) -> int:
