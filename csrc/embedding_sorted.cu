@@ -14,6 +14,7 @@
 // get no gradient (key V, sorted behind all others).
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <utility>
 
 #include "common.cuh"
@@ -512,8 +513,11 @@ sorted_runs_kernel(const uint2* __restrict__ list, long long n, const float* __r
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Entries of a chunk: 8 while that makes no more than 2^15 tasks (the more warps,
-// the shorter their chains of loads), then 32 (fewer parts of cut runs).
-int chunk_of(long long n, int C) { return n * ((C + 255) / 256) <= (8LL << 15) ? 8 : 32; }
+// the shorter their chains of loads), then 32 (fewer parts of cut runs); 32 as
+// well where that makes it one chunk, which cuts no run and saves a launch.
+int chunk_of(long long n, int C) {
+  return n <= 32 || n * ((C + 255) / 256) > (8LL << 15) ? 32 : 8;
+}
 
 }  // namespace
 
@@ -581,8 +585,10 @@ void scaled_embedding_bwd(const void* dout, const unsigned* sorted, void* grad, 
     const bool vec = C % 8 == 0 && aligned16(dout) && aligned16(grad);
     const long long tasks = chunks * slabs;
     const unsigned row_blocks = (unsigned)((tasks + 7) / 8);
-    // units of 256 KB to clear
-    const long long fit = (256LL << 10) / ((long long)C * sizeof(T));
+    // units to clear of 16 to 256 KB, eight a SM where the table allows: a unit
+    // costs a search in the list
+    const long long row = (long long)C * sizeof(T), even = V * row / (8 * kNumSMs);
+    const long long fit = std::min(std::max(even, 16LL << 10), 256LL << 10) / row;
     const int unit = (int)(fit < 1 ? 1 : fit > kUnitRows ? kUnitRows : fit);
     const unsigned units = accumulate ? 0 : (unsigned)((V + unit - 1) / unit);
     auto rows = [&](auto* kernel) {

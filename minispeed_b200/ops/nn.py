@@ -460,7 +460,8 @@ def swiglu(gu: torch.Tensor, save_bits: Optional[int] = None) -> torch.Tensor:
     ``save_bits=8`` keeps ``gu`` for backward in 8 bits (the format of
     :func:`pack_activation`, gate and up in blocks of their own): about half
     the memory of a 16-bit ``gu``.  The output is that of the exact input;
-    the gradient is the formula's at the packed values."""
+    the gradient is the formula's at the packed values (NaN for the values of a
+    block that holds an infinity or a NaN)."""
     if _check_save_bits(save_bits):
         _check_packable(gu)
         if gu.shape[-1] % 2:
@@ -812,8 +813,8 @@ def scaled_embedding(idx: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
                          f"{tuple(weight.shape)}")
     if idx.device != weight.device:
         raise ValueError(f"scaled_embedding: tokens on {idx.device}, table on {weight.device}")
-    if not math.isfinite(scale):
-        raise ValueError(f"scaled_embedding: scale must be finite, got {scale}")
+    if not abs(scale) <= torch.finfo(torch.float32).max:
+        raise ValueError(f"scaled_embedding: scale must be finite in fp32, got {scale}")
     V = weight.shape[0]
     padding = -1
     if padding_idx is not None:

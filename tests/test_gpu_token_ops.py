@@ -83,6 +83,43 @@ def test_logprobs_masks(dtype, V):
     _check_logprobs(x.flip(0), tok.flip(0), T=1.0, k=32, entropy=False)
 
 
+@pytest.mark.parametrize("dtype", DT)
+def test_logprobs_masks_of_rows_shared_by_blocks(dtype):
+    """Few long rows, each read by several blocks: everything that counts in one
+    block's part, in the last values behind its vectors, or nowhere."""
+    V = 40003
+    x = _randn(7, V, seed=2, dtype=dtype, std=3.0)
+    x[0, : V - 3] = -math.inf
+    x[1, 5:] = torch.finfo(dtype).min
+    x[2] = torch.finfo(dtype).min
+    x[3] = -math.inf
+    x[4] = 2.0
+    x[5, 20000:20600] = 9.0                            # more ties than are kept
+    x[6] = -torch.arange(V, device="cuda").to(dtype) / V
+    tok = torch.tensor([V - 1, 0, 7, 8, 9, 20100, -100], device="cuda")
+    for k in (0, 32):
+        _check_logprobs(x, tok, T=1.0, k=k)
+    _check_logprobs(x[:, 1:], (tok - 1).clamp(min=0), T=0.7, k=3)
+
+
+def test_logprobs_alternatives_in_sorted_and_crowded_rows():
+    """Rows whose best values lie beside one another, in one thread's vectors, or
+    all within a narrow band: the threshold lets many through."""
+    V = 128 * 256
+    x = torch.zeros(6, V, device="cuda")
+    x[0] = torch.arange(V, device="cuda") / V
+    x[1] = -torch.arange(V, device="cuda") / V
+    one = (torch.arange(V, device="cuda") // 4 % 256 == 77).float()   # thread 77's fp32 vectors
+    x[2] = one * (1 + torch.arange(V, device="cuda") / V)
+    x[3] = torch.where(one > 0, 1.0, -torch.rand(V, device="cuda", generator=_gen(1)))
+    x[4] = torch.rand(V, device="cuda", generator=_gen(2)).half().float()
+    x[5] = (torch.arange(V, device="cuda") % 7).float()
+    tok = torch.arange(6, device="cuda")
+    for dtype in DT:
+        for k in (1, 8, 32):
+            _check_logprobs(x.to(dtype), tok, k=k)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_logprobs_largest_values(dtype):
     """Finite logits at both ends of the type."""
@@ -172,6 +209,27 @@ def test_logprobs_same_bits_each_time_and_logits_untouched():
     assert torch.equal(x.detach(), kept)
 
 
+def test_logprobs_beyond_32_bit_offsets():
+    """The last rows of logits of more than 2^32 values."""
+    M, V = 33000, 131072
+    x = torch.zeros(M, V, device="cuda", dtype=torch.bfloat16)
+    x[-3:] = _randn(3, V, dtype=torch.bfloat16, std=3.0)
+    x.requires_grad_()
+    tok = torch.full((M,), -100, device="cuda")
+    tok[-3:] = torch.tensor([5, V - 1, 77], device="cuda")
+    tok[0] = 3
+    r = ops.token_logprobs(x, tok, entropy=True, top_k=4)
+    g = _randn(M)
+    (dx,) = torch.autograd.grad(r.logprobs, x, g)
+    want = oracle.logprobs(x[-3:], tok[-3:], k=4, g_lp=g[-3:])
+    oracle.close(r.logprobs[-3:], want["lp"], want["lp_tol"])
+    oracle.close(r.entropy[-3:], want["ent"], want["ent_tol"])
+    assert torch.equal(r.top_tokens[-3:], want["top"])
+    oracle.close(dx[-3:], want["dx"], want["dx_tol"])
+    assert not dx[1:100].any() and not dx[-100:-3].any()
+    assert float(r.logprobs[0].detach()) == pytest.approx(-math.log(V), rel=1e-5)
+
+
 # ------------------------------------------------------- scaled embedding
 def _check_embedding(idx, V, C, dtype, scale=1.0, padding=None, offset=0):
     w = _randn(V * C + offset, seed=C, dtype=dtype)[offset:].view(V, C).requires_grad_()
@@ -210,6 +268,33 @@ def test_embedding_long_runs(dtype, n):
     dw = _check_embedding(mixed, 900, 136, dtype, padding=3)
     assert not dw[3].any()
     assert not _check_embedding(one, 5, 136, dtype, padding=3).any()
+
+
+@pytest.mark.parametrize("n", [1, 8, 33, 5000])
+@pytest.mark.parametrize("V,C", [(3, 8), (70000, 8), (1025, 264), (9, 50000), (4000, 33)])
+def test_embedding_clears_the_other_rows(n, V, C):
+    """Every row of a new gradient is written, whatever was in its memory."""
+    idx = torch.randint(0, V, (n,), device="cuda", generator=_gen(n)) // 2 * 2 % V
+    for _ in range(2):
+        junk = torch.full((V, C), math.nan, device="cuda", dtype=torch.bfloat16)
+        del junk
+        _check_embedding(idx, V, C, torch.bfloat16)
+
+
+def test_embedding_beyond_32_bit_offsets():
+    V, C = 1100000, 4096
+    w = torch.zeros(V, C, device="cuda", dtype=torch.bfloat16)
+    w[-2:] = _randn(2, C, dtype=torch.bfloat16)
+    w.requires_grad_()
+    idx = torch.tensor([V - 1, 0, V - 2, V - 1], device="cuda")
+    y = ops.scaled_embedding(idx, w, 2.0)
+    assert torch.equal(y, (w.detach()[idx].float() * 2).bfloat16())
+    d = _randn(4, C, seed=3, dtype=torch.bfloat16)
+    (dw,) = torch.autograd.grad(y, w, d)
+    assert torch.equal(dw[-1], ((d[0].float() + d[3].float()) * 2).bfloat16())
+    assert torch.equal(dw[-2], (d[2].float() * 2).bfloat16())
+    assert torch.equal(dw[0], (d[1].float() * 2).bfloat16())
+    assert not dw[1:-2].any()
 
 
 @pytest.mark.parametrize("offset", [1, 4])
@@ -511,3 +596,32 @@ def test_engine_on_log_probabilities_and_in_a_graph():
     for other in (runs[1], own):
         assert other == pytest.approx(runs[0], rel=2 ** -8)
     assert all(math.isfinite(v) for v in own)
+
+
+# ------------------------------------------------ the bounds-checked build
+def test_debug_build_records_tokens_out_of_range():
+    """Both builds skip the access; the debug build records it.  The access
+    would have stayed in allocated memory: the tables are parts of larger ones."""
+    import importlib
+
+    from minispeed_b200.ops import _ext
+
+    try:
+        dbg = importlib.import_module("minispeed_b200._C_debug")
+    except ImportError:
+        pytest.skip("debug build not built (MSB_DEBUG_BUILD=1 python setup.py build_ext --inplace)")
+    _ext.bounds_status(reset=True, mod=dbg)
+    V = 100
+    w = _randn(V + 8, 64, dtype=torch.float16)[:V]
+    idx = torch.tensor([3, V + 2, 5, 7], device="cuda")
+    for sort in (False, True):
+        out, _ = dbg.scaled_embedding_fwd(idx, w, 1.0, -1, sort)
+        rec = {r["unit"]: r for r in _ext.bounds_status(reset=True, mod=dbg)}["embedding"]
+        assert (rec["count"], rec["site"], rec["index"], rec["limit"]) == (1, 1, V + 2, V)
+        assert not out[1].any() and torch.equal(out[2], w[5])
+    x = _randn(4, 128)[:, :V]
+    tok = torch.tensor([3, V + 2, -100, 7], device="cuda")
+    lp = dbg.logprob_fwd(x, tok, 1.0, True, 3, -100)[0]
+    rec = {r["unit"]: r for r in _ext.bounds_status(reset=True, mod=dbg)}["logprob"]
+    assert (rec["count"], rec["site"], rec["index"], rec["limit"]) == (1, 8, V + 2, V)
+    assert torch.isnan(lp).tolist() == [False, True, False, False]

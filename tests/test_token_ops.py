@@ -27,6 +27,9 @@ DT = [torch.float32, torch.float16, torch.bfloat16]
     (dict(logits=torch.zeros(2, 99), top_k=33), ValueError),
     (dict(temperature=0.0), ValueError),
     (dict(temperature=math.nan), ValueError),
+    (dict(temperature=-1.0), ValueError),
+    (dict(temperature=1e-31), ValueError),
+    (dict(temperature=math.inf), ValueError),
     (dict(tokens=torch.tensor([1, 5])), IndexError),
     (dict(tokens=torch.tensor([1, -1])), IndexError),
 ])
@@ -42,6 +45,8 @@ def test_token_logprobs_refuses(kw, err):
     (torch.zeros(2, dtype=torch.int64), dict(weight=torch.zeros(3)), ValueError),
     (torch.zeros(2, dtype=torch.int64), dict(weight=torch.zeros(0, 4)), ValueError),
     (torch.zeros(2, dtype=torch.int64), dict(scale=math.inf), ValueError),
+    (torch.zeros(2, dtype=torch.int64), dict(scale=math.nan), ValueError),
+    (torch.zeros(2, dtype=torch.int64), dict(scale=1e39), ValueError),
     (torch.zeros(2, dtype=torch.int64), dict(padding_idx=3), ValueError),
     (torch.tensor([0, 3]), {}, IndexError),
     (torch.tensor([0, -1]), {}, IndexError),
