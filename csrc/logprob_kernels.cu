@@ -356,9 +356,10 @@ __device__ void top_of_part(const Part<T>& p, float my_max, int k, Top& sh) {
   __syncthreads();
 }
 
-// A cluster a row (of one block where there are rows enough).
-template <typename T, bool ENT, bool TOP>
-__global__ void __launch_bounds__(kThreads, 6)
+// A block a row or, SPLIT, a cluster a row where rows are few: then a thread has
+// twice the vectors in flight, as it has few in all.
+template <typename T, bool ENT, bool TOP, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, SPLIT ? 3 : sizeof(T) == 4 ? 4 : 6)
 logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* __restrict__ tok,
                    int V, float c, float inv_t, long long ignore_index, int k,
                    float* __restrict__ logp, float* __restrict__ entropy,
@@ -368,7 +369,7 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   __shared__ Common sh;
   __shared__ std::conditional_t<TOP, Top, int> top;
   cg::cluster_group cluster = cg::this_cluster();
-  const unsigned R = cluster.num_blocks(), q = cluster.block_rank();
+  const unsigned R = SPLIT ? cluster.num_blocks() : 1, q = SPLIT ? cluster.block_rank() : 0;
   const long long r = blockIdx.x / R;
   const T* row = logits + r * ld;
   const int tid = threadIdx.x;
@@ -389,7 +390,7 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   const Part<T> p(row, V, q, R);
 
   Sums a;
-  constexpr int U = 4;   // vectors in flight a thread
+  constexpr int U = SPLIT || sizeof(T) == 4 ? 8 : 4;   // vectors in flight a thread
   for (int v = p.v0 + tid; v < p.v1; v += U * kThreads) {
     Vec<T> x[U];
 #pragma unroll
@@ -408,7 +409,7 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   if constexpr (TOP) top_groups(my_max, k, top);
   __syncthreads();
   float m = reduce_block(sh.buf[0], larger);
-  if (R > 1) {   // the row's maximum
+  if constexpr (SPLIT) {   // the row's maximum
     if (tid == 0) sh.ms[0] = m;
     cluster.sync();
     for (unsigned b = 0; b < R; ++b) m = fmaxf(m, cluster.map_shared_rank(sh.ms, b)[0]);
@@ -430,7 +431,7 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   __syncthreads();
   float s = reduce_block(sh.buf[1], sum), tt = ENT ? reduce_block(sh.buf[2], sum) : 0.f;
   if constexpr (TOP) top_of_part(p, my_max, k, top);
-  if (R > 1) {
+  if constexpr (SPLIT) {
     if (tid == 0) {
       sh.ms[1] = s;
       sh.ms[2] = tt;
@@ -604,7 +605,8 @@ logprob_bwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
 // last rows (182 us with one, 168 with four).
 unsigned blocks_a_row(long long M, int V, int per_vec, int a_sm) {
   unsigned R = 1;
-  while (R < kMaxCluster && M * R < a_sm * kNumSMs && V / (int)(2 * R) >= per_vec * kThreads) R *= 2;
+  while (R < kMaxCluster && M * 2 * R <= a_sm * kNumSMs && V / (int)(2 * R) >= per_vec * kThreads)
+    R *= 2;
   return R;
 }
 
@@ -618,14 +620,18 @@ void logprob_fwd(const void* logits, long long ld, const long long* tok, long lo
   const float inv_t = (float)(1.0 / (double)temperature);
   MSB_DISPATCH_FLOAT(dtype, T, {
     const unsigned R = blocks_a_row(M, V, Vec<T>::N, 2);
-    auto go = [&](auto* kernel) {
-      launch_cluster(R, kernel, (unsigned)M * R, kThreads, 0, st, (const T*)logits, ld, tok, V, c,
-                     inv_t, ignore_index, k, logp, entropy, top_logp, top_tok, stats);
+    auto go = [&](auto ent, auto top) {
+      constexpr bool E = decltype(ent)::value, K = decltype(top)::value;
+      auto run = [&](auto* kernel) {
+        launch_cluster(R, kernel, (unsigned)M * R, kThreads, 0, st, (const T*)logits, ld, tok, V, c,
+                       inv_t, ignore_index, k, logp, entropy, top_logp, top_tok, stats);
+      };
+      R > 1 ? run(logprob_fwd_kernel<T, E, K, true>) : run(logprob_fwd_kernel<T, E, K, false>);
     };
     if (entropy != nullptr) {
-      k > 0 ? go(logprob_fwd_kernel<T, true, true>) : go(logprob_fwd_kernel<T, true, false>);
+      k > 0 ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
     } else {
-      k > 0 ? go(logprob_fwd_kernel<T, false, true>) : go(logprob_fwd_kernel<T, false, false>);
+      k > 0 ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
     }
   });
   MSB_CHECK_LAUNCH("logprob_fwd");
