@@ -50,7 +50,29 @@ struct Vec {
       f[3] = __uint_as_float(r.w);
     }
   }
-  // the largest value that is no NaN (a NaN where all are); two at a time in 16 bits
+  // the larger of this and another, place by place, two at a time in 16 bits; a
+  // NaN only where both are
+  __device__ __forceinline__ Vec larger(const Vec& o) const {
+    Vec m;
+    if constexpr (sizeof(T) == 2) {
+      using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+      const T2 *p = reinterpret_cast<const T2*>(&r), *q = reinterpret_cast<const T2*>(&o.r);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) reinterpret_cast<T2*>(&m.r)[i] = __hmax2(p[i], q[i]);
+    } else {
+      const float *p = reinterpret_cast<const float*>(&r), *q = reinterpret_cast<const float*>(&o.r);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) reinterpret_cast<float*>(&m.r)[i] = fmaxf(p[i], q[i]);
+    }
+    return m;
+  }
+  // -inf everywhere
+  __device__ __forceinline__ void clear() {
+    const unsigned w = sizeof(T) == 4 ? 0xff800000u
+                       : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+    r = make_uint4(w, w, w, w);
+  }
+  // the largest value that is no NaN (a NaN where all are)
   __device__ __forceinline__ float max() const {
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
       const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&r);
@@ -128,7 +150,6 @@ __device__ __forceinline__ void add_z(Sums& a, float2 z) {
 template <typename T, bool ENT>
 __device__ __forceinline__ void add_vec(Sums& a, const Vec<T>& v, float c) {
   constexpr int N = Vec<T>::N;
-  a.see(v.max(), c);
   float x[N];
   v.unpack(x);
   const float2 c2 = make_float2(c, c), r2 = make_float2(-a.ref, -a.ref);
@@ -172,6 +193,12 @@ struct Part {
     return first && i < head ? i : V - tail + i - (first ? head : 0);
   }
 };
+
+__device__ __forceinline__ float max_of_warp(float v) {   // v is no NaN
+  float m;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
 
 // A reduction over the block in two halves, so that several share one barrier.
 template <typename F>
@@ -271,24 +298,17 @@ __device__ void top_of_part(const Part<T>& p, float my_max, int k, Top& sh) {
       if (n < kEqual) sh.equal[n] = key_of(v, i);
     }
   };
-  const int each = (p.v1 - p.v0 + kThreads - 1) / kThreads, items = sh.winners * each;
-  constexpr int U = 4;   // in flight
-  for (int i0 = tid; i0 < items; i0 += U * kThreads) {
-    Vec<T> x[U];
-    int v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * kThreads, w = i / each;
-      v[u] = i < items ? p.v0 + sh.winner[w] + (i - w * each) * kThreads : p.v1;
-      if (v[u] < p.v1) x[u].r = p.mid[v[u]];
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (v[u] >= p.v1 || !(x[u].max() >= thr)) continue;
+  // a warp a winner, a lane a vector of its
+  const int winners = sh.winners;
+  for (int w = warp; w < winners; w += kThreads / 32) {
+    for (int v = p.v0 + sh.winner[w] + lane * kThreads; v < p.v1; v += 32 * kThreads) {
+      Vec<T> x;
+      x.r = p.mid[v];
+      if (!(x.max() >= thr)) continue;
       float f[N];
-      x[u].unpack(f);
+      x.unpack(f);
 #pragma unroll
-      for (int j = 0; j < N; ++j) take(f[j], p.at(v[u]) + j);
+      for (int j = 0; j < N; ++j) take(f[j], p.at(v) + j);
     }
   }
   for (int i = tid; i < p.loose(); i += kThreads) {
@@ -394,8 +414,14 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   for (int v = p.v0 + tid; v < p.v1; v += U * kThreads) {
     Vec<T> x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      x[u].clear();
       if (v + u * kThreads < p.v1) x[u].r = p.mid[v + u * kThreads];
+    }
+    Vec<T> top_of = x[0];
+#pragma unroll
+    for (int u = 1; u < U; ++u) top_of = top_of.larger(x[u]);
+    a.see(top_of.max(), c);
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (v + u * kThreads < p.v1) add_vec<T, ENT>(a, x[u], c);
@@ -405,7 +431,8 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
 
   auto larger = [](float x, float y) { return fmaxf(x, y); };
   auto sum = [](float x, float y) { return x + y; };
-  reduce_warps(my_max, sh.buf[0], larger);
+  const float warp_max = max_of_warp(my_max);
+  if ((tid & 31) == 0) sh.buf[0][tid >> 5] = warp_max;
   if constexpr (TOP) top_groups(my_max, k, top);
   __syncthreads();
   float m = reduce_block(sh.buf[0], larger);
@@ -429,7 +456,11 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   if (ENT) reduce_warps(a.t.x + a.t.y, sh.buf[2], sum);
   if constexpr (TOP) top_threshold(k, top);
   __syncthreads();
-  float s = reduce_block(sh.buf[1], sum), tt = ENT ? reduce_block(sh.buf[2], sum) : 0.f;
+  float s = 0.f, tt = 0.f;
+  if (tid < 32) {   // what the threads that write results need
+    s = reduce_block(sh.buf[1], sum);
+    if (ENT) tt = reduce_block(sh.buf[2], sum);
+  }
   if constexpr (TOP) top_of_part(p, my_max, k, top);
   if constexpr (SPLIT) {
     if (tid == 0) {
