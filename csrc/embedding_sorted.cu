@@ -4,7 +4,7 @@
 //
 // The sum of a row is taken in fp32 in an order that depends on idx alone: the
 // positions are sorted by token (stable, so ascending within a token), the
-// sorted list is cut into chunks of 8 or 32 entries, and every run of one token
+// sorted list is cut into chunks of 32 entries, and every run of one token
 // is summed front to back inside a chunk; a run that crosses chunks leaves one
 // fp32 partial per chunk, added up in chunk order.  No atomics touch values, so
 // the gradient is the same from run to run, and no [V, C] accumulator is kept.
@@ -28,6 +28,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
+// Entries that a warp sums.  With 8, 16384 x 768 naturally distributed tokens took
+// 25 us instead of 27, but 65536 of them 68 instead of 47 and 65536 times one token
+// 385 instead of 88: the shorter the chunks, the more parts of cut runs.
+constexpr int kChunk = 32;
 constexpr int kSortThreads = 1024;
 constexpr int kDigit = 9;           // most bits of a sorting pass
 constexpr int kBins = 1 << kDigit;
@@ -329,7 +333,7 @@ __device__ __forceinline__ void clear_unit(const uint2* __restrict__ list, long 
   }
 }
 
-// A warp sums a chunk of CHUNK sorted entries over 256 columns.  The rows of
+// A warp sums a chunk of the list over 256 columns.  The rows of
 // four entries, and the gradient rows that their sums are added to, are loaded
 // before any is used, whatever runs they belong to: most runs are one or two
 // entries long, and run by run the loads would wait for one another.  open[j]:
@@ -337,7 +341,7 @@ __device__ __forceinline__ void clear_unit(const uint2* __restrict__ list, long 
 //
 // ADD: the sums are added to the rows.  Otherwise the gradient is a new one, and
 // the blocks behind the first `row_blocks` clear the rows of no token meanwhile.
-template <typename T, bool VEC, bool ADD, int CHUNK>
+template <typename T, bool VEC, bool ADD>
 __global__ void __launch_bounds__(256)
 sorted_rows_kernel(const uint2* __restrict__ list, long long n, unsigned V,
                    const T* __restrict__ dout, int C, FastDiv slabs, unsigned tasks, T* grad,
@@ -352,29 +356,29 @@ sorted_rows_kernel(const uint2* __restrict__ list, long long n, unsigned V,
   const unsigned task = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (task >= tasks) return;
   const unsigned j = slabs.div(task);
-  const long long first = (long long)j * CHUNK;
+  const long long first = (long long)j * kChunk;
   const int c0 = (int)(task - j * slabs.d) * 256 + (VEC ? lane * 8 : lane);
-  const int len = (int)min((long long)CHUNK, n - first);
+  const int len = (int)min((long long)kChunk, n - first);
   // lane l: entry l's token; what comes before and behind the chunk
   const uint2 entry = lane < len ? list[first + lane] : make_uint2(V, 0u);
   const unsigned my_key = entry.x, my_pos = entry.y;
   const unsigned prev = first > 0 ? list[first - 1].x : V;
-  const unsigned next = first + CHUNK < n ? list[first + CHUNK].x : V;
+  const unsigned next = first + kChunk < n ? list[first + kChunk].x : V;
   unsigned behind = __shfl_down_sync(0xffffffffu, my_key, 1);   // the key after each entry
-  if (lane == CHUNK - 1) behind = next;
+  if (lane == kChunk - 1) behind = next;
   // entries that are tokens, and those that end a run inside the chunk
   const unsigned live = __ballot_sync(0xffffffffu, lane < len && my_key < V);
   const unsigned ends = __ballot_sync(0xffffffffu, lane < len && my_key < V && behind != my_key);
-  if (c0 == 0) open[j] = live >> (CHUNK - 1) & 1 && !(ends >> (CHUNK - 1) & 1);   // goes on
+  if (c0 == 0) open[j] = live >> (kChunk - 1) & 1 && !(ends >> (kChunk - 1) & 1);   // goes on
   if (live == 0) return;
   const unsigned key0 = __shfl_sync(0xffffffffu, my_key, 0);
   const int head = prev == key0 ? __ffs(~__ballot_sync(0xffffffffu, my_key == key0)) - 1 : 0;
   // `head` entries, when not 0, continue the run of the chunk before (32 of 32: -1)
   const unsigned in_head = prev != key0 ? 0u : head < 0 ? ~0u : (1u << head) - 1u;
-  if (c0 == 0 && (in_head >> (CHUNK - 1) & 1)) open[j] = 0;   // but began earlier
+  if (c0 == 0 && (in_head >> (kChunk - 1) & 1)) open[j] = 0;   // but began earlier
   float a[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 1
-  for (int e0 = 0; e0 < CHUNK; e0 += kRows) {
+  for (int e0 = 0; e0 < kChunk; e0 += kRows) {
     if ((live >> e0) == 0) break;
     Cols<T, VEC> row[kRows], old[ADD ? kRows : 1];
 #pragma unroll
@@ -430,7 +434,7 @@ constexpr int kRunWarps = kRunThreads / 32;
 constexpr int kRunCols = 128;
 constexpr int kLongRun = 24;
 static_assert(kLongRun < 32, "a warp's one look finds the end of a short run");
-template <typename T, bool ADD, bool V4, int CHUNK>
+template <typename T, bool ADD, bool V4>
 __global__ void __launch_bounds__(kRunThreads)
 sorted_runs_kernel(const uint2* __restrict__ list, long long n, const float* __restrict__ part,
                    int C, long long chunks, FastDiv slabs, T* grad, float scale,
@@ -469,8 +473,8 @@ sorted_runs_kernel(const uint2* __restrict__ list, long long n, const float* __r
   for (int t = 0; todo != 0; ++t, todo &= todo - 1) {
     if (t % kRunWarps != warp) continue;
     const int b = __ffs(todo) - 1;
-    const long long j = j0 + b, at = (j + 1 + lane) * CHUNK;   // the chunks behind j
-    const unsigned key = list[j * CHUNK + CHUNK - 1].x;
+    const long long j = j0 + b, at = (j + 1 + lane) * kChunk;   // the chunks behind j
+    const unsigned key = list[j * kChunk + kChunk - 1].x;
     const unsigned other = ~__ballot_sync(0xffffffffu, at < n && list[at].x == key);
     const int count = other == 0 ? 32 : __ffs(other) - 1;
     if (count > kLongRun) {
@@ -484,10 +488,10 @@ sorted_runs_kernel(const uint2* __restrict__ list, long long n, const float* __r
   __syncthreads();
   for (unsigned rest = is_long; rest != 0; rest &= rest - 1) {
     const long long j = j0 + __ffs(rest) - 1;
-    const unsigned key = list[j * CHUNK + CHUNK - 1].x;
+    const unsigned key = list[j * kChunk + kChunk - 1].x;
     long long count = 0;
     for (;;) {
-      const long long at = (j + 1 + count + threadIdx.x) * CHUNK;
+      const long long at = (j + 1 + count + threadIdx.x) * kChunk;
       const int more = __syncthreads_count(at < n && list[at].x == key);
       count += more;
       if (more < kRunThreads) break;
@@ -512,12 +516,13 @@ sorted_runs_kernel(const uint2* __restrict__ list, long long n, const float* __r
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Entries of a chunk: 8 while that makes no more than 2^15 tasks (the more warps,
-// the shorter their chains of loads), then 32 (fewer parts of cut runs); 32 as
-// well where that makes it one chunk, which cuts no run and saves a launch.
-int chunk_of(long long n, int C) {
-  return n <= 32 || n * ((C + 255) / 256) > (8LL << 15) ? 32 : 8;
-}
+long long chunks_of(long long n) { return (n + kChunk - 1) / kChunk; }
+
+// Whether the lookup is launched by itself before the sort.  Beside the sort, a
+// block a SM gathers at 2.6 TB/s of output, by itself the lookup does at 4.2;
+// the sort takes some 9 us and 0.5 us for every 1000 tokens.  65536 x 4096 bf16:
+// 207 us together, 163 apart; 65536 x 768: 43 us together, some 65 apart.
+bool apart(long long n, long long bytes) { return bytes / 7e6 > 9 + n / 1900.0; }
 
 }  // namespace
 
@@ -543,7 +548,9 @@ void scaled_embedding_fwd(const long long* idx, const void* w, void* out, long l
         unsigned R = 1;
         while (R < kMaxCluster && (long long)R * kSortThreads < n) R *= 2;
         // a block a SM in all: 64 registers a thread allow no more
-        const unsigned gather = max(R, grid_for(total, kSortThreads, kNumSMs - R) / R * R);
+        const bool alone = n > most || apart(n, n * C * (long long)sizeof(T));
+        const unsigned gather =
+            alone ? 0 : max(R, grid_for(total, kSortThreads, kNumSMs - R) / R * R);
         uint2 *a = (uint2*)ws, *b = (uint2*)(ws + 2 * n);
         auto go = [&](auto* kernel) {
           check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -554,7 +561,7 @@ void scaled_embedding_fwd(const long long* idx, const void* w, void* out, long l
                          padding, passes, bits, passes & 1 ? a : b, passes & 1 ? b : a);
         };
         vec ? go(lookup_sort_kernel<T, true>) : go(lookup_sort_kernel<T, false>);
-        continue;
+        if (!alone) continue;
       }
       auto go = [&](auto* kernel) {
         launch(kernel, grid_for(total, 256, kNumSMs * 16), 256, 0, st, idx + i, (const T*)w,
@@ -569,7 +576,7 @@ void scaled_embedding_fwd(const long long* idx, const void* w, void* out, long l
 // a flag a chunk, then the parts, 16-byte aligned
 static long long flag_words(long long chunks) { return (chunks + 15) / 16 * 4; }
 long long scaled_embedding_ws(long long n, int C) {
-  const long long chunk = chunk_of(n, C), chunks = (n + chunk - 1) / chunk;
+  const long long chunks = chunks_of(n);
   return flag_words(chunks) + chunks * 2 * C;
 }
 
@@ -577,8 +584,8 @@ void scaled_embedding_bwd(const void* dout, const unsigned* sorted, void* grad, 
                           unsigned* ws, long long n, int C, long long V, float scale, int dtype,
                           cudaStream_t st) {
   const uint2* list = (const uint2*)sorted;
-  const int slabs = (C + 255) / 256, chunk = chunk_of(n, C);
-  const long long chunks = (n + chunk - 1) / chunk;
+  const int slabs = (C + 255) / 256;
+  const long long chunks = chunks_of(n);
   unsigned char* open = (unsigned char*)ws;
   float* part = (float*)(ws + flag_words(chunks));
   MSB_DISPATCH_FLOAT(dtype, T, {
@@ -602,19 +609,12 @@ void scaled_embedding_bwd(const void* dout, const unsigned* sorted, void* grad, 
         launch(kernel, (unsigned)((chunks + 31) / 32 * cols), kRunThreads, 0, st, list, n, part, C,
                chunks, FastDiv(cols), (T*)grad, scale, open);
     };
-    auto go = [&](auto add, auto size) {
+    auto go = [&](auto add) {
       constexpr bool A = decltype(add)::value;
-      constexpr int N = decltype(size)::value;
-      vec ? rows(sorted_rows_kernel<T, true, A, N>) : rows(sorted_rows_kernel<T, false, A, N>);
-      C % 4 == 0 ? runs(sorted_runs_kernel<T, A, true, N>) : runs(sorted_runs_kernel<T, A, false, N>);
+      vec ? rows(sorted_rows_kernel<T, true, A>) : rows(sorted_rows_kernel<T, false, A>);
+      C % 4 == 0 ? runs(sorted_runs_kernel<T, A, true>) : runs(sorted_runs_kernel<T, A, false>);
     };
-    using Short = std::integral_constant<int, 8>;
-    using Long = std::integral_constant<int, 32>;
-    if (accumulate) {
-      chunk == 8 ? go(std::true_type{}, Short{}) : go(std::true_type{}, Long{});
-    } else {
-      chunk == 8 ? go(std::false_type{}, Short{}) : go(std::false_type{}, Long{});
-    }
+    accumulate ? go(std::true_type{}) : go(std::false_type{});
   });
   MSB_CHECK_LAUNCH("scaled_embedding_bwd");
 }
