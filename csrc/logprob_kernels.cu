@@ -33,7 +33,8 @@ constexpr int kMaxCluster = 8;
 constexpr int kGroups = 64;    // groups of threads whose maxima give a threshold, >= kMaxK
 constexpr int kCand = 1024;    // candidates kept above the threshold, and
 constexpr int kEqual = 512;    // at it
-static_assert(kGroups * 4 == kThreads && kMaxK <= kGroups && kMaxK + kEqual <= kCand && kMaxCluster * kMaxK <= kCand, "");
+static_assert(kGroups * 4 == kThreads && kMaxK <= kGroups, "a group is four threads of a warp");
+static_assert(kMaxK + kEqual <= kCand && kMaxCluster * kMaxK <= kCand, "what is ranked fits");
 
 // 16 bytes of logits
 template <typename T>
