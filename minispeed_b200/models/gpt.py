@@ -109,6 +109,8 @@ class GPT(nn.Module):
         With ``targets`` and ``logprobs``, a dict of
         :func:`~minispeed_b200.ops.nn.token_logprobs` options (it may be empty),
         the log probabilities of the targets instead of their mean loss."""
+        if logprobs is not None and targets is None:
+            raise ValueError("logprobs needs targets")
         B, T = idx.shape
         if T > self.block_size:
             raise ValueError(f"sequence length {T} > block_size {self.block_size}")

@@ -125,6 +125,8 @@ class Llama(nn.Module):
     def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None,
                 logprobs: Optional[dict] = None):
         """Logits, mean loss or the targets' log probabilities, as ``GPT.forward``."""
+        if logprobs is not None and targets is None:
+            raise ValueError("logprobs needs targets")
         B, T = idx.shape
         cos, sin = self._tables(T, idx.device)
         if self.config.embed_scale is None:

@@ -9,6 +9,7 @@ import torch.nn as nn
 
 import token_ops_oracle as oracle
 from minispeed_b200.activation_checkpointing import checkpoint
+from minispeed_b200.ops import _ext
 from minispeed_b200.ops import nn as ops
 
 pytestmark = pytest.mark.gpu
@@ -173,6 +174,7 @@ def test_logprobs_token_outside_the_vocabulary():
     assert torch.isnan(r.logprobs).tolist() == [True, False, True]
     (dx,) = torch.autograd.grad(r.logprobs.sum(), x)
     assert not dx[0].any() and not dx[2].any() and dx[1].any()
+    _ext.bounds_status(reset=True)   # the debug build has recorded them
 
 
 def test_logprobs_of_nothing():
@@ -320,6 +322,7 @@ def test_embedding_tokens_outside_the_table():
     want = torch.zeros(50, 16, device="cuda", dtype=torch.float16)
     want[49], want[3] = 4.0, 2.0
     assert torch.equal(dw, want)
+    _ext.bounds_status(reset=True)   # the debug build has recorded them
 
 
 @pytest.mark.parametrize("dtype", DT)
@@ -335,6 +338,27 @@ def test_embedding_adds_into_the_bound_gradient(dtype):
     want, tol = oracle.embedding_grad(d, idx, 700, 0.5, 10, before)
     oracle.close(p.grad, want, tol)
     assert torch.equal(p.grad[200:], before[200:])
+
+
+def test_embedding_gradient_is_the_difference():
+    """As on the CPU: exactly, in whole numbers."""
+    w = torch.randint(-8, 9, (900, 136), device="cuda", generator=_gen(1)).float().requires_grad_()
+    step = torch.randint(-8, 9, (900, 136), device="cuda", generator=_gen(2)).float()
+    idx = torch.randint(0, 900, (3000,), device="cuda", generator=_gen(3)) ** 2 // 900
+    d = torch.randint(-8, 9, (3000, 136), device="cuda", generator=_gen(4)).float()
+    y = ops.scaled_embedding(idx, w, 3.0)
+    (dw,) = torch.autograd.grad(y, w, d)
+    change = ops.scaled_embedding(idx, w.detach() + step, 3.0) - y.detach()
+    assert float((change.double() * d.double()).sum()) == float((dw.double() * step.double()).sum())
+
+
+def test_embedding_backward_twice_from_one_lookup():
+    w = _randn(50, 264).requires_grad_()
+    y = ops.scaled_embedding(torch.randint(0, 50, (500,), device="cuda", generator=_gen(3)), w)
+    d = _randn(500, 264, seed=1)
+    (a,) = torch.autograd.grad(y, w, d, retain_graph=True)
+    (b,) = torch.autograd.grad(y, w, d)
+    assert torch.equal(a, b)
 
 
 def test_embedding_gradient_is_the_same_each_time():
@@ -474,6 +498,21 @@ def test_together_on_a_stream_of_their_own():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_together_on_two_streams_at_once():
+    want = [_all_of_them(_all_state(9)), _all_of_them(_all_state(29))]
+    states = [_all_state(9), _all_state(29)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(3):
+        for st, stream in zip(states, streams):
+            with torch.cuda.stream(stream):
+                got.append(_all_of_them(st))
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(out, want[i % 2]))
+
+
 def test_together_captured_twice_and_replayed_with_new_tokens():
     states = [_all_state(9), _all_state(19)]
     side = torch.cuda.Stream()
@@ -603,8 +642,6 @@ def test_debug_build_records_tokens_out_of_range():
     """Both builds skip the access; the debug build records it.  The access
     would have stayed in allocated memory: the tables are parts of larger ones."""
     import importlib
-
-    from minispeed_b200.ops import _ext
 
     try:
         dbg = importlib.import_module("minispeed_b200._C_debug")

@@ -219,6 +219,39 @@ def test_swiglu_8bit_cpu(dtype, F):
     oracle.close(dx, dw, dt)
 
 
+def test_swiglu_oracle_gradient_is_the_difference_quotient():
+    """At inputs that 8 bits hold exactly, against central differences of the
+    64-bit output: off by h^2 of the third derivatives (under 2 here) and the
+    output's rounding over h."""
+    g = torch.Generator().manual_seed(4)
+    x = torch.randint(-127, 128, (2, 64), generator=g).float() / 32
+    x[:, ::32] = 127 / 32        # every block's largest: the steps are 1 / 32
+    assert torch.equal(oracle.restored(x).float(), x)
+    dh = torch.randn(2, 32, generator=g)
+    _, _, dx, _ = oracle.swiglu(x, dh)
+    h = 1e-5
+    for i in range(0, 64, 7):
+        up, down = x.double(), x.double()
+        up[:, i] += h
+        down[:, i] -= h
+        f = lambda v: (v[:, :32] * torch.sigmoid(v[:, :32]) * v[:, 32:] * dh.double()).sum(-1)  # noqa: E731
+        torch.testing.assert_close((f(up) - f(down)) / (2 * h), dx[:, i], rtol=0, atol=1e-8)
+
+
+def test_scaled_embedding_gradient_is_the_difference():
+    """The lookup is linear: its change with the table is the gradient's product
+    with that change, exactly in whole numbers."""
+    g = torch.Generator().manual_seed(5)
+    w = torch.randint(-8, 9, (13, 6), generator=g).float().requires_grad_()
+    step = torch.randint(-8, 9, (13, 6), generator=g).float()
+    idx = torch.randint(0, 13, (50,), generator=g)
+    d = torch.randint(-8, 9, (50, 6), generator=g).float()
+    y = ops.scaled_embedding(idx, w, 3.0)
+    (dw,) = torch.autograd.grad(y, w, d)
+    change = ops.scaled_embedding(idx, w.detach() + step, 3.0) - y.detach()
+    assert float((change * d).sum()) == float((dw * step).sum())
+
+
 # -------------------------------------------------------- checkpoint
 class _Gate(nn.Module):
     def __init__(self, n):
@@ -312,6 +345,8 @@ def test_model_logprobs_are_the_losses_of_the_targets(which):
     assert r.logprobs.shape == (2, 20) and r.top_tokens.shape == (2, 20, 2)
     torch.testing.assert_close(-r.logprobs.sum() / 38, m(x, targets=y), rtol=1e-5, atol=1e-6)
     assert m(x, targets=y, logprobs={}).entropy is None
+    with pytest.raises(ValueError, match="targets"):
+        m(x, logprobs={})
 
 
 def test_model_options_change_only_what_they_say():
