@@ -138,7 +138,8 @@ const long long* tokens_of(const at::Tensor& t, int64_t n, const at::Tensor& lik
   return reinterpret_cast<const long long*>(t.data_ptr<int64_t>());
 }
 
-// (logprobs [M], entropy [M] or none, top logprobs [M, k], top tokens [M, k], stats [M, 3])
+// (logprobs, entropy or none, top logprobs [..., k], top tokens [..., k], stats [M, 3]), in the
+// tokens' shape
 std::tuple<at::Tensor, OptT, OptT, OptT, at::Tensor> logprob_fwd(
     const at::Tensor& logits, const at::Tensor& tokens, double temperature, bool entropy,
     int64_t k, int64_t ignore_index) {
@@ -149,12 +150,14 @@ std::tuple<at::Tensor, OptT, OptT, OptT, at::Tensor> logprob_fwd(
   TORCH_CHECK(M < (1LL << 31), "too many rows");
   c10::cuda::CUDAGuard g(logits.device());
   const auto f32 = logits.options().dtype(at::kFloat);
-  at::Tensor lp = at::empty({M}, f32), stats = at::empty({M, 3}, f32);
+  at::Tensor lp = at::empty(tokens.sizes(), f32), stats = at::empty({M, 3}, f32);
   OptT ent, tlp, ttok;
-  if (entropy) ent = at::empty({M}, f32);
+  if (entropy) ent = at::empty(tokens.sizes(), f32);
   if (k > 0) {
-    tlp = at::empty({M, k}, f32);
-    ttok = at::empty({M, k}, logits.options().dtype(at::kLong));
+    auto shape = tokens.sizes().vec();
+    shape.push_back(k);
+    tlp = at::empty(shape, f32);
+    ttok = at::empty(shape, logits.options().dtype(at::kLong));
   }
   msb::logprob_fwd(logits.data_ptr(), row_stride(logits), tok, M, (int)V, (float)temperature,
                    ignore_index, (int)k, lp.data_ptr<float>(),
@@ -187,8 +190,8 @@ at::Tensor logprob_bwd(const at::Tensor& logits, const at::Tensor& tokens, const
   const long long* tt = nullptr;
   c10::cuda::CUDAGuard g(logits.device());
   if (given(top_tokens) && given(g_top)) {
-    TORCH_CHECK(top_tokens->dim() == 2 && top_tokens->size(1) <= 32, "top tokens: [M, k]");
-    k = top_tokens->size(1);
+    TORCH_CHECK(top_tokens->dim() >= 1 && top_tokens->size(-1) <= 32, "top tokens: [..., k]");
+    k = top_tokens->size(-1);
     tt = tokens_of(*top_tokens, M * k, logits);
   }
   const at::Tensor gl = grad_f32(g_logp, M, logits), ge = grad_f32(g_ent, M, logits),
@@ -278,20 +281,17 @@ struct TokenLogprobs : public Function<TokenLogprobs> {
                                int64_t k, int64_t ignore_index) {
     const at::Tensor rows = as_rows(logits), tok = tokens.contiguous();
     auto [lp, ent, tlp, ttok, stats] = logprob_fwd(rows, tok, temperature, entropy, k, ignore_index);
-    variable_list out;
-    auto shape = tokens.sizes().vec();
-    out.push_back(lp.view(shape));
-    if (entropy) out.push_back(ent->view(shape));
+    variable_list out = {lp};
+    if (entropy) out.push_back(*ent);
     if (k > 0) {
-      shape.push_back(k);
-      out.push_back(tlp->view(shape));
-      out.push_back(ttok->view(shape));
+      out.push_back(*tlp);
+      out.push_back(*ttok);
     }
     if (ctx != nullptr) {
       ctx->set_materialize_grads(false);
       if (k > 0) ctx->mark_non_differentiable({out.back()});
       ctx->save_for_backward({rows, tok, k > 0 ? *ttok : at::Tensor(), stats});
-      ctx->saved_data["shape"] = logits.sizes().vec();
+      if (logits.dim() != 2) ctx->saved_data["shape"] = logits.sizes().vec();
       ctx->saved_data["temperature"] = temperature;
       ctx->saved_data["entropy"] = entropy;
       ctx->saved_data["ignore_index"] = ignore_index;
@@ -309,8 +309,9 @@ struct TokenLogprobs : public Function<TokenLogprobs> {
       const auto saved = ctx->get_saved_variables();
       dx = logprob_bwd(saved[0], saved[1], some(saved[2]), saved[3], some(gl), some(ge), some(gt),
                        ctx->saved_data["temperature"].toDouble(),
-                       ctx->saved_data["ignore_index"].toInt())
-               .view(ctx->saved_data["shape"].toIntVector());
+                       ctx->saved_data["ignore_index"].toInt());
+      const auto shape = ctx->saved_data.find("shape");
+      if (shape != ctx->saved_data.end()) dx = dx.view(shape->second.toIntVector());
     }
     return {dx, none, none, none, none, none};
   }
