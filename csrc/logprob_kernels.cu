@@ -269,19 +269,22 @@ __device__ __forceinline__ void top_groups(float my_max, int k, Top& sh) {
   if (tid == 0) sh.winners = sh.above = sh.at = 0;
 }
 __device__ __forceinline__ void top_threshold(int k, Top& sh) {
-  const int tid = threadIdx.x;
-  if (tid >= kGroups) return;
-  const unsigned mine = sh.group[tid];
+  // four threads a group, each against a quarter of the groups
+  const int g = threadIdx.x >> 2, part = threadIdx.x & 3;
+  const unsigned mine = sh.group[g];
   int r = 0;
-#pragma unroll 4
-  for (int j = 0; j < kGroups; j += 4) {
+#pragma unroll
+  for (int i = 0; i < kGroups / 16; ++i) {
+    const int j = (i * 4 + part) * 4;
     const uint4 o = *reinterpret_cast<const uint4*>(sh.group + j);
-    r += o.x > mine || (o.x == mine && j < tid);
-    r += o.y > mine || (o.y == mine && j + 1 < tid);
-    r += o.z > mine || (o.z == mine && j + 2 < tid);
-    r += o.w > mine || (o.w == mine && j + 3 < tid);
+    r += o.x > mine || (o.x == mine && j < g);
+    r += o.y > mine || (o.y == mine && j + 1 < g);
+    r += o.z > mine || (o.z == mine && j + 2 < g);
+    r += o.w > mine || (o.w == mine && j + 3 < g);
   }
-  if (r == k - 1) sh.threshold = value_of(mine);
+  r += __shfl_xor_sync(0xffffffffu, r, 1);
+  r += __shfl_xor_sync(0xffffffffu, r, 2);
+  if (r == k - 1 && part == 0) sh.threshold = value_of(mine);
 }
 template <typename T>
 __device__ void top_of_part(const Part<T>& p, float my_max, int k, Top& sh) {
