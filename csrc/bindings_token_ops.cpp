@@ -33,7 +33,9 @@ void check_contig(const at::Tensor& t, const char* name) {
 
 void check_matrix(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
-  TORCH_CHECK(t.dim() == 2 && t.stride(1) == 1 && (t.size(0) <= 1 || t.stride(0) >= t.size(1)),
+  // (an axis of one element may have any stride)
+  TORCH_CHECK(t.dim() == 2 && (t.stride(1) == 1 || t.size(1) == 1) &&
+                  (t.size(0) <= 1 || t.stride(0) >= t.size(1)),
               name, " must be a row-major matrix (unit column stride)");
   TORCH_CHECK(t.size(1) > 0 && t.size(1) < std::numeric_limits<int>::max() - 1024, name,
               " is too wide");
@@ -271,7 +273,9 @@ OptT some(const at::Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
 // `t` as rows of its last axis with unit column stride; copied where no view is
 at::Tensor as_rows(const at::Tensor& t) {
   at::Tensor m = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
-  return m.stride(1) != 1 || (m.size(0) > 1 && m.stride(0) < m.size(1)) ? m.contiguous() : m;
+  const bool rows = (m.stride(1) == 1 || m.size(1) == 1) &&
+                    (m.size(0) <= 1 || m.stride(0) >= m.size(1));
+  return rows ? m : m.contiguous();
 }
 
 struct TokenLogprobs : public Function<TokenLogprobs> {

@@ -386,7 +386,7 @@ __device__ void top_of_part(const Part<T>& p, float my_max, int k, Top& sh) {
 //
 // Bound in 16 bits by DRAM, the exponentials (XU pipe 74%) and issue (70%)
 // together: 8192 x 50257 fp16, a tenth of it ignored, 119 us (6.2 TB/s, 0.95 of
-// the copy rate), with the entropy 125, with 8 alternatives 147; 2048 x 128256
+// the copy rate), with the entropy 125, with 8 alternatives 139; 2048 x 128256
 // bf16 90, 92, 109.
 template <typename T, bool ENT, bool TOP, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : sizeof(T) == 4 ? 4 : 6)

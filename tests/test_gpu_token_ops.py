@@ -369,6 +369,18 @@ def test_embedding_gradient_is_the_same_each_time():
     assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])
 
 
+def test_one_column_with_any_stride():
+    """An axis of one element may have any stride."""
+    x = _randn(1, 9)
+    for v in (x.T, x.T.unsqueeze(1), _randn(9, 5)[:, 2:3], x[:, :1].expand(9, 1)):
+        assert torch.equal(ops.pack_activation(v).unpack(), oracle.restored(v).float())
+        _check_logprobs(v, torch.zeros(v.shape[:-1], dtype=torch.int64, device="cuda"), k=1)
+    w = x.T.detach().requires_grad_()
+    y = ops.scaled_embedding(torch.tensor([3, 3, 8], device="cuda"), w, 2.0)
+    (dw,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    assert dw[:, 0].tolist() == [0, 0, 0, 4, 0, 0, 0, 0, 2]
+
+
 # ------------------------------------------------------ 8-bit activations
 def _awkward(dtype, rows, D, seed=0):
     x = _randn(rows, D, seed=seed) * torch.exp(_randn(rows, 1, seed=seed + 1) * 4)
