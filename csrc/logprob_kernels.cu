@@ -108,13 +108,16 @@ __device__ __forceinline__ int key_index(unsigned long long k) {
 
 // The exponents of a row are z = x c - m c, one fused operation on the rounded
 // product m c (the same one wherever the row's z are computed, so its rounding
-// cancels).  Where m c comes near fp32's range (the lowest value of fp32 or bf16
-// is a common mask) the row is `wide` and z = (x - m) c.
+// cancels).  That rounding shifts them by up to 2^-24 |m c|: where |m c| reaches
+// 2^24 (a mask of -1e9 is not far from it, the lowest value of fp32 beyond fp32's
+// range) the row is `wide` and z = (x - m) c.  A reference is held to that range:
+// values that lie below it count nothing in a row that is not wide.
+constexpr float kWide = 16777216.f;
 __device__ __forceinline__ bool is_wide(float m, float c) {
-  return fabsf(m * c) >= 1e37f && m != -INFINITY;
+  return fabsf(m * c) >= kWide && m != -INFINITY;
 }
 __device__ __forceinline__ float reference(float m, float c) {   // of -inf: 0
-  return m == -INFINITY ? 0.f : fminf(fmaxf(m * c, -1e37f), 1e37f);
+  return m == -INFINITY ? 0.f : fminf(fmaxf(m * c, -kWide), kWide);
 }
 
 // exponents at or under this give 2^z = 0; a larger one in z's place keeps

@@ -85,6 +85,36 @@ def test_logprobs_masks(dtype, V):
 
 
 @pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("V", [50, 3001, 40003])
+def test_logprobs_masks_of_any_size(dtype, V):
+    """Masks from -1e4 to -1e38, and offsets of as much above zero: in part of a
+    row, for whole threads, in all of it."""
+    sizes = [v for v in (1e4, 1e6, 3e7, 1e9, 1e10, 1e20, 1e30, 1e38)
+             if v < torch.finfo(dtype).max]
+    x = _randn(4 * len(sizes), V, seed=2, dtype=dtype, std=3.0)
+    for i, v in enumerate(sizes):
+        x[4 * i, torch.rand(V, device="cuda", generator=_gen(i)) < 0.95] = -v
+        x[4 * i + 1, 8:] = -v
+        x[4 * i + 2] = -v
+        x[4 * i + 2, 3] = -2 * v if 2 * v < torch.finfo(dtype).max else -v
+        x[4 * i + 3, V // 2:] = v
+    tok = torch.arange(4 * len(sizes), device="cuda") % 7
+    _check_logprobs(x, tok, k=3)
+    _check_logprobs(x, tok, T=0.3, k=0)
+
+
+def test_logprobs_temperatures_at_their_limits():
+    x = _randn(3, 300, seed=2)
+    tok = x.argmax(-1)
+    r = ops.token_logprobs(x, tok, temperature=1e-30, entropy=True, top_k=2)
+    assert r.logprobs.tolist() == [0, 0, 0] and r.entropy.tolist() == [0, 0, 0]
+    assert bool((r.top_logprobs[:, 1] < -1e25).all())
+    r = ops.token_logprobs(x, tok, temperature=1e30, entropy=True)
+    assert r.logprobs.tolist() == pytest.approx([-math.log(300)] * 3, rel=1e-6)
+    assert r.entropy.tolist() == pytest.approx([math.log(300)] * 3, rel=1e-6)
+
+
+@pytest.mark.parametrize("dtype", DT)
 def test_logprobs_masks_of_rows_shared_by_blocks(dtype):
     """Few long rows, each read by several blocks: everything that counts in one
     block's part, in the last values behind its vectors, or nowhere."""

@@ -35,9 +35,9 @@ def logprobs(x, tok, T=1.0, k=0, ignore=-100, g_lp=None, g_ent=None, g_top=None)
     out = {"lp": settle(logp.gather(1, at), -math.inf)[:, 0], "ent": settle(H, 0.0)[:, 0],
            "top_lp": settle(logp.gather(1, top), -math.inf), "top": torch.where(on, top, -1)}
     # the exponent of every term that counts is off by a few half steps of |x| / T
-    # (of nothing where |x| is so large that differences are taken first), a sum of
-    # V terms over at least 256 running sums by V / 256 half steps, exp2 by four
-    counts = (logp > -100) & (x64.abs() < 1e30)
+    # (of nothing where that reaches 2^24 ln 2 and differences are taken first), a sum
+    # of V terms over at least 256 running sums by V / 256 half steps, exp2 by four
+    counts = (logp > -100) & (x64.abs() / T < 2 ** 24 * math.log(2))
     size = torch.where(counts, x64.abs(), 0.0).amax(-1, keepdim=True) / T
     tol = U32 * (V / 256 + 64 + 16 * size)
     # a log probability is itself rounded, and a difference of logits before it
