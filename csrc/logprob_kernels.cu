@@ -507,9 +507,11 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   const float l2 = log2f(s);
   auto value = [&](float x) {
     if (empty) return -INFINITY;
-    const float z = fmaf(x, c, -ref);
-    // far below the maximum, z may overflow where the difference does not
-    return wide || z < -1e30f ? (x - m) * inv_t - kLn2 * l2 : kLn2 * (z - l2);
+    const float z = fmaf(x, c, -ref), d = x - m;
+    if (!wide && !(z < -1e30f)) return kLn2 * (z - l2);
+    // far below the maximum, z may overflow where the difference does not, and the
+    // difference where its quotient does not
+    return (d == -INFINITY && x != -INFINITY ? x * inv_t - m * inv_t : d * inv_t) - kLn2 * l2;
   };
   if (tid == 0) {
     (void)MSB_OK(in, kSiteLogprobToken, t, V);

@@ -161,6 +161,7 @@ def test_logprobs_largest_values(dtype):
     x[2] = big
     x[3, 9] = 0.0
     _check_logprobs(x, torch.tensor([5, 6, 70, 9], device="cuda"), k=4)
+    _check_logprobs(x, torch.tensor([6, 0, 0, 0], device="cuda"), T=2.5, k=7)
 
 
 @pytest.mark.parametrize("bad", [math.inf, math.nan])

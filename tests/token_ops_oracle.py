@@ -57,7 +57,9 @@ def logprobs(x, tok, T=1.0, k=0, ignore=-100, g_lp=None, g_ent=None, g_top=None)
     out["dx"] = torch.where(on & ~empty, dx, 0.0)
     scale = (hot.abs() + p * (gl.abs() + gt.abs().sum(-1, keepdim=True)
                               + ge.abs() * (live.abs() + H + 1))) / T
-    out["dx_tol"] = (half_step(dtype) * out["dx"].abs() + 4 * (tol + k * U32) * scale
+    # exp2 of an exponent under -126 is 0
+    flushed = 2.0 ** -126 * (gl.abs() + gt.abs().sum(-1, keepdim=True) + ge.abs() * (130 + H)) / T
+    out["dx_tol"] = (half_step(dtype) * out["dx"].abs() + 4 * (tol + k * U32) * scale + flushed
                      + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps)
     return out
 
