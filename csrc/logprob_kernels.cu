@@ -34,7 +34,7 @@ constexpr int kGroups = 64;    // groups of threads whose maxima give a threshol
 constexpr int kCand = 1024;    // candidates kept above the threshold, and
 constexpr int kEqual = 512;    // at it
 static_assert(kGroups * 4 == kThreads && kMaxK <= kGroups, "a group is four threads of a warp");
-static_assert(kMaxK + kEqual <= kCand && kMaxCluster * kMaxK <= kCand, "what is ranked fits");
+static_assert(kMaxK + kEqual <= kCand, "what is ranked fits");
 
 // 16 bytes of logits
 template <typename T>
@@ -66,6 +66,11 @@ struct Vec {
       for (int i = 0; i < 4; ++i) reinterpret_cast<float*>(&m.r)[i] = fmaxf(p[i], q[i]);
     }
     return m;
+  }
+  // a load that stays where it stands in the program
+  __device__ __forceinline__ void load(const uint4* p) {
+    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
   }
   // -inf everywhere
   __device__ __forceinline__ void clear() {
@@ -219,10 +224,17 @@ __device__ __forceinline__ float reduce_block(const float* buf, F&& f) {   // af
   return v;
 }
 
-// What a block knows of its part of the row, read by the cluster's first block.
-struct Common {
-  float ms[3];                         // maximum, s, t
-  float buf[3][kThreads / 32];
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// What the blocks of a row write into the first one's memory.
+struct alignas(16) Joined {
+  unsigned long long best[kMaxCluster * kMaxK];
+  float m[kMaxCluster], s[kMaxCluster], t[kMaxCluster];
 };
 struct alignas(16) Top {
   unsigned long long best[kMaxK];      // its alternatives, best first; 0: none
@@ -399,13 +411,33 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
                    float* __restrict__ top_logp, long long* __restrict__ top_tok,
                    float* __restrict__ stats) {
   ::msb::pdl_begin();
-  __shared__ Common sh;
+  __shared__ float buf[3][kThreads / 32];
   __shared__ std::conditional_t<TOP, Top, int> top;
+  __shared__ std::conditional_t<SPLIT, Joined, int> joined;
   cg::cluster_group cluster = cg::this_cluster();
   const unsigned R = SPLIT ? cluster.num_blocks() : 1, q = SPLIT ? cluster.block_rank() : 0;
   const long long r = blockIdx.x / R;
   const T* row = logits + r * ld;
   const int tid = threadIdx.x;
+  const Part<T> p(row, V, q, R);
+  constexpr int U = SPLIT || sizeof(T) == 4 ? 8 : 4;   // vectors in flight a thread
+  Vec<T> x[U];
+  auto load = [&](int v) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      x[u].clear();
+      if (v + u * kThreads >= p.v1) continue;
+      if constexpr (SPLIT) {
+        x[u].load(p.mid + v + u * kThreads);
+      } else {
+        x[u].r = p.mid[v + u * kThreads];
+      }
+    }
+  };
+  if constexpr (SPLIT) {
+    load(p.v0 + tid);   // on its way while the token is
+    cluster_arrive();   // waited for before the first block's memory is written
+  }
   const long long t = tok[r];
   if (t == ignore_index) {   // in all blocks of the cluster alike
     if (q == 0 && tid == 0) {
@@ -420,17 +452,10 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   }
   const bool in = t >= 0 && t < V;
   const float xt = q == 0 && tid == 0 && in ? to_f32(row[t]) : 0.f;
-  const Part<T> p(row, V, q, R);
 
   Sums a;
-  constexpr int U = SPLIT || sizeof(T) == 4 ? 8 : 4;   // vectors in flight a thread
   for (int v = p.v0 + tid; v < p.v1; v += U * kThreads) {
-    Vec<T> x[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      x[u].clear();
-      if (v + u * kThreads < p.v1) x[u].r = p.mid[v + u * kThreads];
-    }
+    if (!SPLIT || v != p.v0 + tid) load(v);
     Vec<T> top_of = x[0];
 #pragma unroll
     for (int u = 1; u < U; ++u) top_of = top_of.larger(x[u]);
@@ -445,17 +470,12 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   auto larger = [](float x, float y) { return fmaxf(x, y); };
   auto sum = [](float x, float y) { return x + y; };
   const float warp_max = max_of_warp(my_max);
-  if ((tid & 31) == 0) sh.buf[0][tid >> 5] = warp_max;
+  if ((tid & 31) == 0) buf[0][tid >> 5] = warp_max;
   if constexpr (TOP) top_groups(my_max, k, top);
   __syncthreads();
-  float m = reduce_block(sh.buf[0], larger);
-  if constexpr (SPLIT) {   // the row's maximum
-    if (tid == 0) sh.ms[0] = m;
-    cluster.sync();
-    for (unsigned b = 0; b < R; ++b) m = fmaxf(m, cluster.map_shared_rank(sh.ms, b)[0]);
-  }
-  const bool wide = is_wide(m, c);
-  const float ref = reference(m, c);
+  float m = reduce_block(buf[0], larger);   // of the block's part
+  bool wide = is_wide(m, c);
+  float ref = reference(m, c);
   if (wide && m != INFINITY) {   // once more, with differences
     a.s = a.t = make_float2(0.f, 0.f);
     for (int i = p.at(p.v0) + tid; i < p.at(p.v1); i += kThreads)
@@ -465,40 +485,50 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
   } else {
     a.rebase(ref);
   }
-  reduce_warps(a.s.x + a.s.y, sh.buf[1], sum);
-  if (ENT) reduce_warps(a.t.x + a.t.y, sh.buf[2], sum);
+  reduce_warps(a.s.x + a.s.y, buf[1], sum);
+  if (ENT) reduce_warps(a.t.x + a.t.y, buf[2], sum);
   if constexpr (TOP) top_threshold(k, top);
   __syncthreads();
   float s = 0.f, tt = 0.f;
   if (tid < 32) {   // what the threads that write results need
-    s = reduce_block(sh.buf[1], sum);
-    if (ENT) tt = reduce_block(sh.buf[2], sum);
+    s = reduce_block(buf[1], sum);
+    if (ENT) tt = reduce_block(buf[2], sum);
   }
   if constexpr (TOP) top_of_part(p, my_max, k, top);
   if constexpr (SPLIT) {
+    cluster_wait();   // the first block runs
+    Joined* to = cluster.map_shared_rank(&joined, 0);
     if (tid == 0) {
-      sh.ms[1] = s;
-      sh.ms[2] = tt;
+      to->m[q] = m;
+      to->s[q] = s;
+      to->t[q] = tt;
     }
-    cluster.sync();
-    if (q == 0) {
-      s = tt = 0.f;
-      for (unsigned b = 0; b < R; ++b) {
-        const float* o = cluster.map_shared_rank(sh.ms, b);
-        s += o[1];
-        tt += o[2];
-      }
-      if constexpr (TOP) {
-        for (int i = tid; i < (int)R * k; i += kThreads)
-          top.cand[i] = cluster.map_shared_rank(top.best, i / k)[i % k];
-      }
+    if constexpr (TOP) {
+      if (tid < k) to->best[q * k + tid] = top.best[tid];
     }
-    cluster.sync();   // the other blocks' shared memory has been read
+    cluster_arrive();
     if (q != 0) return;
+    cluster_wait();
+    // the parts' sums, each relative to its own maximum, relative to the row's
+    m = joined.m[0];
+    for (unsigned b = 1; b < R; ++b) m = fmaxf(m, joined.m[b]);
+    wide = is_wide(m, c);
+    ref = reference(m, c);
+    s = tt = 0.f;
+    for (unsigned b = 0; b < R; ++b) {
+      const float mb = joined.m[b], rb = reference(mb, c);
+      const bool wb = is_wide(mb, c);
+      // what a part's exponents lack of the row's
+      float d = wide ? (mb - m) * c - (wb ? 0.f : fmaf(mb, c, -rb)) : wb ? kLowZ : rb - ref;
+      d = mb == -INFINITY ? 0.f : fmaxf(d, kLowZ);
+      const float f = ex2_approx(d);
+      s += f * joined.s[b];
+      tt += f * fmaf(joined.s[b], d, joined.t[b]);
+    }
     if constexpr (TOP) {
       if (tid < k) top.best[tid] = 0;
       __syncthreads();
-      rank_keys(top.cand, (int)R * k, top.best, k);
+      rank_keys(joined.best, (int)R * k, top.best, k);
       __syncthreads();
     }
   }
@@ -646,11 +676,11 @@ logprob_bwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
 }
 
 // Blocks a row: up to `a_sm` a SM in all where rows are few, as long as a block has
-// two vectors a thread.  The forward's blocks wait for one another, and more than
-// it takes to fill the GPU cost more than they bring (96 x 128256 bf16 with 20
-// alternatives: 29 us with one, 21 with two or four, 35 with eight; 2048 rows with
-// their entropy: 92 us with one, 119 with two).  The backward's are independent,
-// and even out the last rows (2048 rows: 172 us with one, 162 with two).
+// two vectors a thread.  The forward's blocks wait for one another: as many as are
+// resident together, no more (96 x 128256 bf16 with 20 alternatives, in a graph:
+// 21 us with one, 15 with two or four, 23 with eight; 2048 rows with their entropy:
+// 92 us with one, 119 with two).  The backward's are independent, and even out the
+// last rows (2048 rows: 172 us with one, 162 with two).
 unsigned blocks_a_row(long long M, int V, int per_vec, int a_sm) {
   unsigned R = 1;
   while (R < kMaxCluster && M * 2 * R <= a_sm * kNumSMs && V / (int)(2 * R) >= per_vec * kThreads)
@@ -667,7 +697,7 @@ void logprob_fwd(const void* logits, long long ld, const long long* tok, long lo
   const float c = (float)(1.4426950408889634 / (double)temperature);
   const float inv_t = (float)(1.0 / (double)temperature);
   MSB_DISPATCH_FLOAT(dtype, T, {
-    const unsigned R = blocks_a_row(M, V, Vec<T>::N, 2);
+    const unsigned R = blocks_a_row(M, V, Vec<T>::N, 3);
     auto go = [&](auto ent, auto top) {
       constexpr bool E = decltype(ent)::value, K = decltype(top)::value;
       auto run = [&](auto* kernel) {
