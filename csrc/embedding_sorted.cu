@@ -333,11 +333,11 @@ __device__ __forceinline__ void clear_unit(const uint2* __restrict__ list, long 
   }
 }
 
-// A warp sums a chunk of the list over 256 columns.  The rows of
-// four entries, and the gradient rows that their sums are added to, are loaded
-// before any is used, whatever runs they belong to: most runs are one or two
-// entries long, and run by run the loads would wait for one another.  open[j]:
-// a run begins in chunk j and goes on behind it.
+// A warp sums a chunk of the list over 256 columns.  The rows of four entries, and
+// the gradient rows that their sums are added to, are loaded before any is used,
+// whatever runs they belong to: most runs are one or two entries long, and run by
+// run the loads would wait for one another.  open[j]: a run begins in chunk j and
+// goes on behind it.
 //
 // ADD: the sums are added to the rows.  Otherwise the gradient is a new one, and
 // the blocks behind the first `row_blocks` clear the rows of no token meanwhile.
@@ -411,12 +411,8 @@ sorted_rows_kernel(const uint2* __restrict__ list, long long n, unsigned V,
         }
         Cols<T, VEC>::store(grad + (long long)k * C, c0, C, f);
       } else {   // a part: slot 0 continues the chunk before, slot 1 begins here
-        float* d = part + ((long long)j * 2 + (in_head >> e & 1 ? 0 : 1)) * C;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int c = VEC ? c0 + i : c0 + 32 * i;
-          if (c < C) d[c] = a[i];
-        }
+        Cols<float, VEC>::store(part + ((long long)j * 2 + (in_head >> e & 1 ? 0 : 1)) * C, c0, C,
+                                a);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) a[i] = 0.f;
