@@ -30,7 +30,7 @@ namespace cg = cooperative_groups;
 
 // Entries that a warp sums.  With 8, 16384 x 768 naturally distributed tokens took
 // 25 us instead of 27, but 65536 of them 68 instead of 47 and 65536 times one token
-// 385 instead of 88: the shorter the chunks, the more parts of cut runs.
+// 385 instead of 86: the shorter the chunks, the more parts of cut runs.
 constexpr int kChunk = 32;
 constexpr int kSortThreads = 1024;
 constexpr int kDigit = 9;           // most bits of a sorting pass
