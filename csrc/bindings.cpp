@@ -448,7 +448,9 @@ std::pair<int, int> tune_gemm(const at::Tensor& a, const at::Tensor& b, int a_mn
   std::pair<int, int> pick = cands[0];
   for (auto& c : cands) {
     float t = 1e30f;
-    for (int rep = 0; rep < 3; ++rep) {
+    // Short products are timed eight times instead of twice: one disturbed pair of
+    // times made a split plan win, whose sums round differently from other runs'.
+    for (int rep = 0; rep < (t < 0.2f || rep < 2 ? 9 : 3); ++rep) {
       cuda_ok(cudaEventRecord(e0, st), "event");
       msb::gemm_tcgen05(a.data_ptr(), a.stride(0), a_mn, b.data_ptr(), b.stride(0), b_mn,
                         scratch.data_ptr(), ldn, nullptr, (int)M, (int)N, (int)K, dtype_code(a), 0,
