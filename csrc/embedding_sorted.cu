@@ -101,11 +101,12 @@ __device__ __forceinline__ void lookup(const long long* __restrict__ idx,
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const unsigned i = i0 + u * threads;
-      const unsigned m = i < total ? per.div(i) : 0u;
-      const int c = (int)(i - m * per.d) * (VEC ? 8 : 1);
-      const long long t = i < total ? idx[m] : -1;
+      const bool live = i < total;   // a place behind the end has column 0 of no token
+      const unsigned m = live ? per.div(i) : 0u;
+      const int c = live ? (int)(i - m * per.d) * (VEC ? 8 : 1) : 0;
+      const long long t = live ? idx[m] : -1;
       const bool in = t >= 0 && t < V;
-      if (c == 0 && i < total) (void)MSB_OK(in, kSiteEmbeddingToken, t, V);
+      if (c == 0 && live) (void)MSB_OK(in, kSiteEmbeddingToken, t, V);
       if constexpr (VEC) {
         v[u].load(w + (in ? t : 0) * C, c, in ? C : 0);   // zeros where not in
       } else {

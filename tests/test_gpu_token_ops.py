@@ -330,6 +330,18 @@ def test_embedding_beyond_32_bit_offsets():
     assert not dw[1:-2].any()
 
 
+def test_embedding_lookup_of_more_than_2_31_values():
+    """Places behind the end of a launch's last round, whose number times eight
+    passes 31 bits, read nothing."""
+    n, V, C = 600001, 37, 4096
+    w = _randn(V, C, dtype=torch.bfloat16)
+    idx = torch.randint(0, V, (n,), device="cuda", generator=_gen(1))
+    y = ops.scaled_embedding(idx, w, 2.0)
+    want = (w.float() * 2).bfloat16()
+    for i in range(0, n, 100000):
+        assert torch.equal(y[i:i + 100000], want[idx[i:i + 100000]])
+
+
 @pytest.mark.parametrize("offset", [1, 4])
 def test_embedding_unaligned(offset):
     idx = torch.randint(0, 40, (3, 50), device="cuda", generator=_gen(1))
