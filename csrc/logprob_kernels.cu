@@ -115,8 +115,10 @@ __device__ __forceinline__ int key_index(unsigned long long k) {
 // product m c (the same one wherever the row's z are computed, so its rounding
 // cancels).  That rounding shifts them by up to 2^-24 |m c|: where |m c| reaches
 // 2^24 (a mask of -1e9 is not far from it, the lowest value of fp32 beyond fp32's
-// range) the row is `wide` and z = (x - m) c.  A reference is held to that range:
-// values that lie below it count nothing in a row that is not wide.
+// range) the row is `wide` and z = (x - m) c.  A reference is held to that range, so
+// a thread whose values all lie below it sums them relative to its lower end, next
+// to which they still count; a block of a shared row whose own part is wide sums it
+// relative to the part's maximum.
 constexpr float kWide = 16777216.f;
 __device__ __forceinline__ bool is_wide(float m, float c) {
   return fabsf(m * c) >= kWide && m != -INFINITY;
@@ -518,8 +520,10 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* 
     for (unsigned b = 0; b < R; ++b) {
       const float mb = joined.m[b], rb = reference(mb, c);
       const bool wb = is_wide(mb, c);
-      // what a part's exponents lack of the row's
-      float d = wide ? (mb - m) * c - (wb ? 0.f : fmaf(mb, c, -rb)) : wb ? kLowZ : rb - ref;
+      // what a part's exponents lack of the row's: from the difference of the maxima
+      // where either is wide, each with what its reference lacks of it
+      const float of_part = wb ? 0.f : fmaf(mb, c, -rb), of_row = wide ? 0.f : fmaf(m, c, -ref);
+      float d = wide || wb ? (mb - m) * c - of_part + of_row : rb - ref;
       d = mb == -INFINITY ? 0.f : fmaxf(d, kLowZ);
       const float f = ex2_approx(d);
       s += f * joined.s[b];

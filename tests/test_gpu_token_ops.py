@@ -164,6 +164,35 @@ def test_logprobs_largest_values(dtype):
     _check_logprobs(x, torch.tensor([6, 0, 0, 0], device="cuda"), T=2.5, k=7)
 
 
+@pytest.mark.parametrize("copies", [1, 40])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_logprobs_at_the_limit_of_wide_rows(sign, copies):
+    """Logits on both sides of 2^24 / log2(e), where differences are taken before
+    the scaling: parts of rows shared by blocks (few rows) or read by one block
+    (many).  A shift changes no probability, so the values are those of the
+    small distances from the limit, which fp32 holds exactly here."""
+    V, limit = 40003, sign * 11629080
+    half = torch.arange(V, device="cuda") < V // 2
+    step = [torch.randint(0, 20, (V,), device="cuda", generator=_gen(i)) for i in range(4)]
+    rows = [torch.where(half, 0, 1), torch.where(half, 1, 0), torch.where(half, -step[0], 3 - step[1]),
+            -step[2], 1 - step[3], torch.where(half, -1, 0)]
+    rows[3][-1] = 2          # alone above the limit, behind the vectors of the last block
+    off = torch.stack(rows).repeat(copies, 1).float()
+    n = len(off)
+    x = (off + limit).requires_grad_()
+    assert torch.equal(x.detach() - limit, off)
+    tok = torch.arange(n, device="cuda") * 7919 % V
+    r = ops.token_logprobs(x, tok, entropy=True, top_k=3)
+    gs = [_randn(n, seed=1), _randn(n, seed=2), _randn(n, 3, seed=3)]
+    want = oracle.logprobs(off, tok, k=3, g_lp=gs[0], g_ent=gs[1], g_top=gs[2])
+    oracle.close(r.logprobs, want["lp"], want["lp_tol"])
+    oracle.close(r.entropy, want["ent"], want["ent_tol"])
+    assert torch.equal(r.top_tokens, want["top"])
+    oracle.close(r.top_logprobs, want["top_lp"], want["top_tol"])
+    (dx,) = torch.autograd.grad([r.logprobs, r.entropy, r.top_logprobs], x, gs)
+    oracle.close(dx, want["dx"], want["dx_tol"])
+
+
 @pytest.mark.parametrize("bad", [math.inf, math.nan])
 @pytest.mark.parametrize("V", [77, 5000])
 def test_logprobs_not_finite(bad, V):
