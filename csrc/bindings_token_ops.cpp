@@ -266,7 +266,13 @@ using torch::autograd::AutogradContext;
 using torch::autograd::Function;
 using torch::autograd::variable_list;
 
-bool wants_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+// Whether `t` needs a node in the graph.  Forward-mode tangents have no kernels:
+// without a node they would be lost, so they are refused here.
+bool wants_grad(const at::Tensor& t, const char* op) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), op,
+                              ": forward-mode derivatives are not implemented on CUDA");
+  return at::GradMode::is_enabled() && t.requires_grad();
+}
 
 OptT some(const at::Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
 
@@ -323,7 +329,7 @@ struct TokenLogprobs : public Function<TokenLogprobs> {
 
 variable_list token_logprobs(const at::Tensor& logits, const at::Tensor& tokens,
                              double temperature, bool entropy, int64_t k, int64_t ignore_index) {
-  if (wants_grad(logits))
+  if (wants_grad(logits, "token_logprobs"))
     return TokenLogprobs::apply(logits, tokens, temperature, entropy, k, ignore_index);
   return TokenLogprobs::forward(nullptr, logits, tokens, temperature, entropy, k, ignore_index);
 }
@@ -364,7 +370,8 @@ struct ScaledEmbedding : public Function<ScaledEmbedding> {
 // `sink`: weight is a parameter, whose gradient is added to in place where it has one
 at::Tensor scaled_embedding(const at::Tensor& idx, const at::Tensor& weight, double scale,
                             int64_t padding, bool sink) {
-  if (wants_grad(weight)) return ScaledEmbedding::apply(idx, weight, scale, padding, sink);
+  if (wants_grad(weight, "scaled_embedding"))
+    return ScaledEmbedding::apply(idx, weight, scale, padding, sink);
   return ScaledEmbedding::forward(nullptr, idx, weight, scale, padding, sink);
 }
 
@@ -382,7 +389,7 @@ struct SwiGLU8 : public Function<SwiGLU8> {
 };
 
 at::Tensor swiglu8(const at::Tensor& gu) {
-  return wants_grad(gu) ? SwiGLU8::apply(gu) : SwiGLU8::forward(nullptr, gu);
+  return wants_grad(gu, "swiglu with save_bits=8") ? SwiGLU8::apply(gu) : SwiGLU8::forward(nullptr, gu);
 }
 
 std::tuple<at::Tensor, at::Tensor> pack_rows(const at::Tensor& x) {

@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 import torch.nn as nn
 
 import token_ops_oracle as oracle
@@ -549,6 +550,28 @@ def test_checkpoint_8bit_cuda_random_state_and_gradient():
     xr = oracle.restored(leaf.detach()).to(leaf.dtype)
     want = torch.where(y == 0, torch.zeros_like(xr), 4 * xr)   # 2 x / (1 - 0.5)
     assert torch.equal(leaf.grad, want)
+
+
+# ------------------------------------------- derivatives without a kernel
+_DIFFERENTIABLE = {
+    "token_logprobs": (lambda x: ops.token_logprobs(x, torch.arange(3, device="cuda")).logprobs, (3, 8)),
+    "scaled_embedding": (lambda w: ops.scaled_embedding(torch.tensor([1, 2, 1], device="cuda"), w), (5, 8)),
+    "swiglu": (lambda x: ops.swiglu(x, save_bits=8), (3, 16)),
+}
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("op", _DIFFERENTIABLE)
+def test_forward_mode_is_refused(op, grad):
+    call, shape = _DIFFERENTIABLE[op]
+    x = _randn(*shape).requires_grad_(grad)
+    with fwad.dual_level():
+        dual = fwad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(dual)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            call(dual)
+        assert torch.equal(call(fwad.unpack_dual(dual).primal), call(x))
 
 
 # ----------------------------------------------- streams, graphs, together
