@@ -274,6 +274,13 @@ bool wants_grad(const at::Tensor& t, const char* op) {
   return at::GradMode::is_enabled() && t.requires_grad();
 }
 
+// The gradients come from kernels and have no graph of their own: under
+// create_graph they would count as constants.
+void first_derivative_only(const char* op) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), op,
+                              ": second derivatives (create_graph=True) are not implemented on CUDA");
+}
+
 OptT some(const at::Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
 
 // `t` as rows of its last axis with unit column stride; copied where no view is
@@ -310,6 +317,7 @@ struct TokenLogprobs : public Function<TokenLogprobs> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    first_derivative_only("token_logprobs");
     const bool entropy = ctx->saved_data["entropy"].toBool();
     const at::Tensor none, &gl = g[0], &ge = entropy ? g[1] : none;
     const size_t top = entropy ? 2 : 1;
@@ -350,6 +358,7 @@ struct ScaledEmbedding : public Function<ScaledEmbedding> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    first_derivative_only("scaled_embedding");
     const at::Tensor none;
     const at::Tensor dout = g[0].contiguous();
     OptT sink;
@@ -383,6 +392,7 @@ struct SwiGLU8 : public Function<SwiGLU8> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    first_derivative_only("swiglu with save_bits=8");
     const auto saved = ctx->get_saved_variables();
     return {swiglu8_bwd(g[0].contiguous(), saved[0], saved[1])};
   }

@@ -461,7 +461,8 @@ def swiglu(gu: torch.Tensor, save_bits: Optional[int] = None) -> torch.Tensor:
     :func:`pack_activation`, gate and up in blocks of their own): about half
     the memory of a 16-bit ``gu``.  The output is that of the exact input;
     the gradient is the formula's at the packed values (NaN for the values of a
-    block that holds an infinity or a NaN).  Forward-mode derivatives raise."""
+    block that holds an infinity or a NaN).  Forward-mode derivatives raise, on
+    CUDA second ones too."""
     if _check_save_bits(save_bits):
         _check_packable(gu)
         if gu.shape[-1] % 2:
@@ -682,7 +683,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
 
     Gradients flow to ``logits`` from the log probabilities, the entropy and
     the top log probabilities.  Unlike :func:`cross_entropy` this leaves the
-    logits as they are.  Forward-mode derivatives raise on CUDA."""
+    logits as they are.  Second and forward-mode derivatives raise on CUDA."""
     if logits.dtype not in _DTYPE_CODES:
         raise TypeError(f"token_logprobs: fp32, fp16 or bf16 logits, got {logits.dtype}")
     if tokens.dtype != torch.int64:
@@ -804,7 +805,7 @@ def scaled_embedding(idx: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
 
     A token outside the table raises ``IndexError`` on the CPU; on CUDA it
     reads as a zero row and gives no gradient, as in :func:`embedding`.
-    Forward-mode derivatives raise."""
+    Forward-mode derivatives raise, on CUDA second ones too."""
     if idx.dtype != torch.int64:
         raise TypeError(f"scaled_embedding: int64 tokens, got {idx.dtype}")
     if weight.dtype not in _DTYPE_CODES:

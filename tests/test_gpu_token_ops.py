@@ -574,6 +574,27 @@ def test_forward_mode_is_refused(op, grad):
         assert torch.equal(call(fwad.unpack_dual(dual).primal), call(x))
 
 
+@pytest.mark.parametrize("op", _DIFFERENTIABLE)
+def test_second_derivatives_are_refused(op):
+    call, shape = _DIFFERENTIABLE[op]
+    x = _randn(*shape).requires_grad_()
+    y = call(x * 1)
+    (dx,) = torch.autograd.grad(y.sum(), x, retain_graph=True)
+    with pytest.raises(NotImplementedError, match="create_graph"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+    assert torch.equal(torch.autograd.grad(y.sum(), x)[0], dx)
+
+
+def test_second_derivatives_leave_the_bound_gradient_alone():
+    p = nn.Parameter(_randn(5, 8))
+    p.grad = _randn(5, 8, seed=1)
+    before = p.grad.clone()
+    y = ops.scaled_embedding(torch.tensor([1, 2, 1], device="cuda"), p)
+    with pytest.raises(NotImplementedError, match="create_graph"):
+        y.sum().backward(create_graph=True)
+    assert torch.equal(p.grad, before)
+
+
 # ----------------------------------------------- streams, graphs, together
 def _all_of_them(st):
     h = ops.scaled_embedding(st["idx"], st["table"], 3.0, padding_idx=0)
