@@ -434,6 +434,9 @@ class _SwiGLU8CPU(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dh):
+        if torch.is_grad_enabled():   # the packed values have no graph back to gu
+            raise NotImplementedError("swiglu with save_bits=8: second derivatives "
+                                      "(create_graph=True) are not implemented")
         F_ = dh.shape[-1]
         g, u = _unpack8_torch(*ctx.saved_tensors, F_).view(-1, 2, F_).unbind(1)
         d = dh.reshape(-1, F_).float()
@@ -461,8 +464,8 @@ def swiglu(gu: torch.Tensor, save_bits: Optional[int] = None) -> torch.Tensor:
     :func:`pack_activation`, gate and up in blocks of their own): about half
     the memory of a 16-bit ``gu``.  The output is that of the exact input;
     the gradient is the formula's at the packed values (NaN for the values of a
-    block that holds an infinity or a NaN).  Forward-mode derivatives raise, on
-    CUDA second ones too."""
+    block that holds an infinity or a NaN).  Second and forward-mode derivatives
+    raise."""
     if _check_save_bits(save_bits):
         _check_packable(gu)
         if gu.shape[-1] % 2:

@@ -219,6 +219,15 @@ def test_swiglu_8bit_cpu(dtype, F):
     oracle.close(dx, dw, dt)
 
 
+@pytest.mark.parametrize("of_dh", [False, True])
+def test_swiglu_8bit_cpu_refuses_second_derivatives(of_dh):
+    x = torch.randn(2, 64, requires_grad=True)
+    dh = torch.randn(2, 32, requires_grad=of_dh)
+    h = ops.swiglu(x, save_bits=8)
+    with pytest.raises(NotImplementedError, match="create_graph"):
+        torch.autograd.grad(h, x, dh, create_graph=True)
+
+
 def test_swiglu_oracle_gradient_is_the_difference_quotient():
     """At inputs that 8 bits hold exactly, against central differences of the
     64-bit output: off by h^2 of the third derivatives (under 2 here) and the
