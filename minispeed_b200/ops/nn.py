@@ -790,7 +790,7 @@ class _ScaledEmbeddingCPU(torch.autograd.Function):
         (idx,) = ctx.saved_tensors
         padding, scale = ctx.args
         idx = idx.reshape(-1)
-        rows = dout.reshape(idx.numel(), -1).float() * scale
+        rows = dout.reshape(idx.numel(), dout.shape[-1]).float() * scale
         rows = torch.where((idx == padding)[:, None], 0.0, rows)
         dw = torch.zeros(ctx.weight.shape).index_add_(0, idx, rows)
         return None, dw.to(dout.dtype), None, None

@@ -145,6 +145,15 @@ def test_scaled_embedding_cpu(dtype):
     oracle.close(dw, want, tol)
 
 
+@pytest.mark.parametrize("shape", [(0,), (2, 0), (0, 3)])
+def test_scaled_embedding_cpu_of_nothing(shape):
+    w = torch.randn(5, 4, requires_grad=True)
+    y = ops.scaled_embedding(torch.zeros(shape, dtype=torch.int64), w, 2.0)
+    assert y.shape == (*shape, 4)
+    (dw,) = torch.autograd.grad(y.sum(), w)
+    assert torch.equal(dw, torch.zeros(5, 4))
+
+
 def test_scaled_embedding_cpu_uses_the_sink_or_autograd():
     p = nn.Parameter(torch.randn(6, 4))
     p.grad = torch.ones(6, 4)
