@@ -30,19 +30,33 @@ class _Saved8:
 
     def __init__(self, args):
         self.exact = args
-        self.saved = [pack_activation(a) if self._activation(a) else a for a in args]
+        self.saved = [(pack_activation(a), self._layout(a)) if self._activation(a) else (a, None)
+                      for a in args]
 
     @staticmethod
     def _activation(a) -> bool:
         return (isinstance(a, torch.Tensor) and a.requires_grad and not a.is_leaf
                 and a.dtype in (torch.float32, torch.float16, torch.bfloat16) and a.dim() > 0)
 
+    @staticmethod
+    def _layout(a):
+        """The strides of a dense tensor whose axes lie in the order of ``a``'s;
+        None where that is contiguous."""
+        return None if a.is_contiguous() else torch.empty_like(a, device="meta").stride()
+
+    @staticmethod
+    def _restore(packed, layout):
+        x = packed.unpack()
+        if layout is not None and layout != x.stride():
+            x = torch.empty_strided(x.shape, layout, dtype=x.dtype, device=x.device).copy_(x)
+        return x.requires_grad_()
+
     def take(self):
         if self.exact is not None:
             args, self.exact = self.exact, None
             return args
-        return [a.unpack().requires_grad_() if isinstance(a, PackedActivation) else a
-                for a in self.saved]
+        return [self._restore(a, layout) if isinstance(a, PackedActivation) else a
+                for a, layout in self.saved]
 
 
 def checkpoint(function, *args, **kwargs):
@@ -52,8 +66,9 @@ def checkpoint(function, *args, **kwargs):
     ``save_bits=8`` also packs the activations among ``args`` (tensors that
     require a gradient and are not leaves) to 8 bits between the two runs.  The
     outputs are those of the exact arguments; the recompute, and so the
-    gradients, start from the packed ones.  Tensors inside containers and
-    keyword arguments are kept as they are."""
+    gradients, start from the packed ones: dense tensors with the axes in the
+    order of the arguments', each argument a tensor of its own.  Tensors inside
+    containers and keyword arguments are kept as they are."""
     save_bits = kwargs.pop("save_bits", None)
     use_reentrant = kwargs.pop("use_reentrant", False)
     if not _check_save_bits(save_bits) or not torch.is_grad_enabled():

@@ -336,6 +336,32 @@ def test_checkpoint_8bit_keeps_the_random_state():
     assert torch.equal(leaf.grad != 0, y.detach() != 0)
 
 
+@pytest.mark.parametrize("order", [(1, 0, 2), (0, 2, 1), (2, 1, 0)])
+def test_checkpoint_8bit_keeps_the_order_of_axes(order):
+    """A transposed argument is one in the recompute too: the function may rely
+    on a view of it."""
+    back = [order.index(i) for i in range(3)]
+    leaf = torch.randn(3, 4, 32, requires_grad=True)
+
+    def flat_cube(t):
+        return (t.permute(back).view(12, 32) ** 3).sum()
+
+    checkpoint(flat_cube, (leaf * 1).permute(order), save_bits=8).backward()
+    moved = leaf.detach().permute(order)     # its blocks lie along its own last axis
+    want = 3 * oracle.restored(moved).float().permute(back) ** 2
+    torch.testing.assert_close(leaf.grad, want, rtol=1e-6, atol=0)
+
+
+def test_checkpoint_8bit_of_views_that_are_not_dense():
+    base = torch.randn(5, 8, 64, requires_grad=True)
+    for view in (lambda t: t[:, ::2, :40], lambda t: t[:1].expand(3, 8, 64),
+                 lambda t: t.transpose(0, 1)[..., ::2]):
+        x = view(base * 1)
+        y = checkpoint(lambda t: (t * t).sum(), x, save_bits=8)
+        (got,) = torch.autograd.grad(y, x)
+        assert torch.equal(got, 2 * oracle.restored(x.detach()).float())
+
+
 def test_checkpoint_8bit_twice_backward():
     leaf = torch.randn(4, 32, requires_grad=True)
     y = checkpoint(lambda t: (t * t).sum(), leaf * 1, save_bits=8)
