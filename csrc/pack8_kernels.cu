@@ -263,14 +263,24 @@ unpack8_any_kernel(const unsigned* __restrict__ codes, const unsigned char* __re
   }
 }
 
-// sigmoid(g); 0 where e^-g overflows
-__device__ __forceinline__ float sigmoid_f(float g) {
-  return rcp_approx(1.f + ex2_approx(g * -kLog2e));
+// sigmoid(g); 0 where e^-g overflows.  In 16 bits by approximations whose error,
+// some 2^-24 |g| of the value, is far below the result's half step of 2^-11 or
+// 2^-8 of it (in quarters, as the reciprocal of a number from 2^126 on is flushed
+// to 0, and bf16 has values that small); fp32 has no such room and takes the
+// exponential and the quotient that SwiGLU without 8-bit saves does.
+template <typename T>
+__device__ __forceinline__ float sigmoid_of(float g) {
+  return sizeof(T) == 4 ? 1.f / (1.f + expf(-g))
+                        : 0.25f * rcp_approx(fmaf(0.25f, ex2_approx(g * -kLog2e), 0.25f));
 }
-__device__ __forceinline__ float silu_f(float g) { return g * sigmoid_f(g); }
+template <typename T>
+__device__ __forceinline__ float silu_of(float g) {
+  return sizeof(T) == 4 ? g / (1.f + expf(-g)) : g * sigmoid_of<T>(g);
+}
 // h = silu(g) u:  dg = dh u s (1 + g (1 - s)),  du = dh g s,  s = sigmoid(g)
+template <typename T>
 __device__ __forceinline__ void swiglu_grad(float dh, float g, float u, float& dg, float& du) {
-  const float s = sigmoid_f(g), t = dh * s;
+  const float s = sigmoid_of<T>(g), t = dh * s;
   dg = t * u * fmaf(g, 1.f - s, 1.f);
   du = t * g;
 }
@@ -326,7 +336,7 @@ swiglu8_fwd_vec_kernel(const T* __restrict__ gu, T* __restrict__ h, uint2* __res
       }
       if (i < total && c < F) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) g[k] = silu_f(g[k]) * u[k];
+        for (int k = 0; k < 8; ++k) g[k] = silu_of<T>(g[k]) * u[k];
         store_eight(h + (long long)row * F + c, g);
       }
     }
@@ -364,7 +374,7 @@ swiglu8_bwd_vec_kernel(const T* __restrict__ dh, const uint2* __restrict__ codes
       values8(wg[j], code_scale(bg[j]), g);
       values8(wu[j], code_scale(bu[j]), u);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) swiglu_grad(d[k], g[k], u[k], g[k], u[k]);
+      for (int k = 0; k < 8; ++k) swiglu_grad<T>(d[k], g[k], u[k], g[k], u[k]);
       T* p = dgu + (long long)row * 2 * F + c;
       store_eight(p, g);
       store_eight(p + F, u);
@@ -398,7 +408,7 @@ swiglu8_fwd_any_kernel(const T* __restrict__ gu, T* __restrict__ h, unsigned* __
       }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) g.f[k] = silu_f(g.f[k]) * u.f[k];
+    for (int k = 0; k < 4; ++k) g.f[k] = silu_of<T>(g.f[k]) * u.f[k];
     g.store(h + (long long)row * F + c, left);
   }
 }
@@ -419,7 +429,7 @@ swiglu8_bwd_any_kernel(const T* __restrict__ dh, const unsigned* __restrict__ co
     g.values(codes[at], code_scale(scales[at >> 3]));
     u.values(codes[at + nq.d], code_scale(scales[(at + nq.d) >> 3]));
 #pragma unroll
-    for (int k = 0; k < 4; ++k) swiglu_grad(d.f[k], g.f[k], u.f[k], g.f[k], u.f[k]);
+    for (int k = 0; k < 4; ++k) swiglu_grad<T>(d.f[k], g.f[k], u.f[k], g.f[k], u.f[k]);
     T* p = dgu + (long long)row * 2 * F + c;
     g.store(p, left);
     u.store(p + F, left);

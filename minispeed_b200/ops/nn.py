@@ -462,8 +462,9 @@ def swiglu(gu: torch.Tensor, save_bits: Optional[int] = None) -> torch.Tensor:
 
     ``save_bits=8`` keeps ``gu`` for backward in 8 bits (the format of
     :func:`pack_activation`, gate and up in blocks of their own): about half
-    the memory of a 16-bit ``gu``.  The output is that of the exact input;
-    the gradient is the formula's at the packed values (NaN for the values of a
+    the memory of a 16-bit ``gu``.  The output is that of the exact input: in
+    fp32 the same bits as without, in 16 bits now and then the next value.  The
+    gradient is the formula's at the packed values (NaN for the values of a
     block that holds an infinity or a NaN).  Second and forward-mode derivatives
     raise."""
     if _check_save_bits(save_bits):

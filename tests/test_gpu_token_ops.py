@@ -515,6 +515,25 @@ def test_swiglu_8bit(dtype, rows, F):
     oracle.close(dx, dw, dt)
 
 
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("F", [64, 45])
+def test_swiglu_8bit_output_is_the_plain_one(dtype, F):
+    """Gates from the one end of the exponential's range to the other.  In fp32
+    bit for bit the output of SwiGLU without 8-bit saves; in 16 bits rounded
+    from within 2^-16 of it, so at most one step apart (and a subnormal one)."""
+    g = torch.linspace(-100, 100, 300 * F, device="cuda").view(300, F).to(dtype)
+    u = _randn(300, F, seed=1, dtype=dtype)
+    even = torch.cat([nn.functional.pad(v, (0, -F % 8)) for v in (g, u)], -1)   # its widths
+    want = ops.swiglu(even)[:, :F]
+    h = ops.swiglu(torch.cat([g, u], -1), save_bits=8)
+    if dtype == torch.float32:
+        assert torch.equal(h, want)
+    else:
+        f = torch.finfo(dtype)
+        off = (h.double() - want.double()).abs()
+        assert bool((off <= f.eps * want.double().abs() + f.smallest_normal * f.eps).all())
+
+
 def test_swiglu_8bit_layouts_and_nothing():
     base = _randn(4, 6, 300, dtype=torch.bfloat16).requires_grad_()
     for x in (base[..., 1:129], base.transpose(0, 1), base[:, ::2, :64], base[:, :0]):
