@@ -74,6 +74,17 @@ def test_8bit_refusals():
         checkpoint(torch.sin, torch.zeros(3), save_bits=8, use_reentrant=True)
 
 
+def test_backward_kernels_are_reached_through_their_forward_only():
+    """They trust the sizes and lists that their forward left: a list of tokens
+    read for a table of another size would name rows that are not there."""
+    from minispeed_b200.ops import _ext
+
+    mod = _ext.load()
+    assert hasattr(mod, "token_logprobs") and hasattr(mod, "scaled_embedding")
+    for name in ("logprob_bwd", "scaled_embedding_bwd", "swiglu8_bwd", "swiglu8_fwd", "pack8"):
+        assert not hasattr(mod, name)
+
+
 # ---------------------------------------------------- CPU definitions
 def _logits(dtype, seed=0):
     g = torch.Generator().manual_seed(seed)
