@@ -277,12 +277,14 @@ template <typename T>
 __device__ __forceinline__ float silu_of(float g) {
   return sizeof(T) == 4 ? g / (1.f + expf(-g)) : g * sigmoid_of<T>(g);
 }
-// h = silu(g) u:  dg = dh u s (1 + g (1 - s)),  du = dh g s,  s = sigmoid(g)
+// h = silu(g) u:  dg = dh u s (1 + g (1 - s)),  du = dh g s,  s = sigmoid(g).
+// The smallest factor is s; times dh alone it may be subnormal where the results
+// are not.
 template <typename T>
 __device__ __forceinline__ void swiglu_grad(float dh, float g, float u, float& dg, float& du) {
-  const float s = sigmoid_of<T>(g), t = dh * s;
-  dg = t * u * fmaf(g, 1.f - s, 1.f);
-  du = t * g;
+  const float s = sigmoid_of<T>(g);
+  dg = dh * u * (s * fmaf(g, 1.f - s, 1.f));
+  du = dh * (g * s);
 }
 
 // gu rows are [gate (F) | up (F)]; the two halves are packed as rows 2r and

@@ -441,7 +441,7 @@ class _SwiGLU8CPU(torch.autograd.Function):
         g, u = _unpack8_torch(*ctx.saved_tensors, F_).view(-1, 2, F_).unbind(1)
         d = dh.reshape(-1, F_).float()
         s = torch.sigmoid(g)
-        dgu = torch.cat([d * u * s * (1 + g * (1 - s)), d * g * s], -1)
+        dgu = torch.cat([d * u * (s * (1 + g * (1 - s))), d * (g * s)], -1)
         return dgu.view(*dh.shape[:-1], 2 * F_).to(dh.dtype)
 
 

@@ -534,6 +534,21 @@ def test_swiglu_8bit_output_is_the_plain_one(dtype, F):
         assert bool((off <= f.eps * want.double().abs() + f.smallest_normal * f.eps).all())
 
 
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("F", [64, 45])
+def test_swiglu_8bit_gates_far_from_zero(dtype, F):
+    """Down to the last gates whose sigmoid fp32 holds in full, with small
+    upstream gradients."""
+    x = torch.cat([torch.linspace(-87, 87, 300 * F, device="cuda").view(300, F),
+                   40 * _randn(300, F)], -1).to(dtype).requires_grad_()
+    dh = _randn(300, F, seed=3, dtype=dtype, std=2.0 ** -12)
+    h = ops.swiglu(x, save_bits=8)
+    hw, ht, dw, dt = oracle.swiglu(x.detach(), dh)
+    oracle.close(h, hw, ht)
+    (dx,) = torch.autograd.grad(h, x, dh)
+    oracle.close(dx, dw, dt)
+
+
 def test_swiglu_8bit_layouts_and_nothing():
     base = _randn(4, 6, 300, dtype=torch.bfloat16).requires_grad_()
     for x in (base[..., 1:129], base.transpose(0, 1), base[:, ::2, :64], base[:, :0]):

@@ -239,6 +239,19 @@ def test_swiglu_8bit_cpu(dtype, F):
     oracle.close(dx, dw, dt)
 
 
+@pytest.mark.parametrize("dtype", DT)
+def test_swiglu_8bit_cpu_gates_far_from_zero(dtype):
+    """As on the GPU: down to the last gates whose sigmoid fp32 holds in full."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.cat([torch.linspace(-87, 87, 300 * 45).view(300, 45),
+                   40 * torch.randn(300, 45, generator=g)], -1).to(dtype).requires_grad_()
+    dh = (torch.randn(300, 45, generator=g) * 2.0 ** -12).to(dtype)
+    h = ops.swiglu(x, save_bits=8)
+    (dx,) = torch.autograd.grad(h, x, dh)
+    _, _, dw, dt = oracle.swiglu(x.detach(), dh)
+    oracle.close(dx, dw, dt)
+
+
 @pytest.mark.parametrize("of_dh", [False, True])
 def test_swiglu_8bit_cpu_refuses_second_derivatives(of_dh):
     x = torch.randn(2, 64, requires_grad=True)
