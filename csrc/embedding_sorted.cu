@@ -2,12 +2,13 @@
 //
 //   out[i] = scale * W[idx_i]        dW[v] = scale * sum over {i : idx_i = v} of dout[i]
 //
-// The sum of a row is taken in fp32 in an order that depends on idx alone: the
-// positions are sorted by token (stable, so ascending within a token), the
-// sorted list is cut into chunks of 32 entries, and every run of one token
-// is summed front to back inside a chunk; a run that crosses chunks leaves one
-// fp32 partial per chunk, added up in chunk order.  No atomics touch values, so
-// the gradient is the same from run to run, and no [V, C] accumulator is kept.
+// The sum of a row is taken in fp32 in an order that depends on the tokens of the
+// call alone: the positions are sorted by token (stable, so ascending within a
+// token), the sorted list of all tokens is cut into chunks of 32 entries, and every
+// run of one token is summed front to back inside a chunk; a run that crosses
+// chunks leaves one fp32 partial per chunk, added up in chunk order (by eighths of
+// the chunks where there are many).  No atomics touch values, so the gradient is
+// the same from run to run, and no [V, C] accumulator is kept.
 //
 // The lookup sorts for the backward pass on one cluster while the other SMs
 // gather.  Tokens outside [0, V) read as a zero row; they and the padding token

@@ -401,10 +401,11 @@ __device__ void top_of_part(const Part<T>& p, float my_max, int k, Top& sh) {
 // twice the vectors in flight, as it has few in all; in fp32 as well, where a
 // vector is half the work (1021 x 32003: 29 us, 33 with four and more blocks).
 //
-// Bound in 16 bits by DRAM, the exponentials (XU pipe 74%) and issue (70%)
-// together: 8192 x 50257 fp16, a tenth of it ignored, 119 us (6.2 TB/s, 0.95 of
-// the copy rate), with the entropy 125, with 8 alternatives 139; 2048 x 128256
-// bf16 90, 92, 109.
+// Bound in 16 bits by DRAM: 8192 x 50257 fp16, a tenth of it ignored, 119 us (6.2
+// TB/s, 0.95 of the copy rate; XU pipe 75%, issue slots 56%), with the entropy 125,
+// with 8 alternatives 139; 2048 x 128256 bf16 90, 92, 109.  The alternatives add
+// their second look and its barriers, when nothing is at its limit (DRAM 0.85 of the
+// copy rate, XU pipe 60%, issue slots 59%).
 template <typename T, bool ENT, bool TOP, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, SPLIT ? 3 : sizeof(T) == 4 ? 4 : 6)
 logprob_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* __restrict__ tok,

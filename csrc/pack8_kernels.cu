@@ -139,8 +139,8 @@ struct Scale {
 // The vector kernels: widths that are a multiple of 8 and 16-byte aligned rows,
 // four lanes a block, eight values a lane.  A thread has two vectors in flight,
 // a grid's width apart.  The number of vectors of a launch fits 31 bits.
-// Bound by DRAM: swiglu8 at 4096 x 14336 bf16 moves its 473 MB in 76 us forward
-// and 77 us backward, 6.2 TB/s.
+// Bound by DRAM: swiglu8 at 4096 x 14336 bf16 moves its 473 MB in 77 us forward
+// and 80 us backward, 6.1 and 5.9 TB/s.
 constexpr int kThreads = 256;
 constexpr int kFlight = 2;
 
@@ -203,7 +203,9 @@ unpack8_vec_kernel(const uint2* __restrict__ codes, const unsigned char* __restr
 }
 
 // Any width, stride and alignment: eight lanes a block, four values a lane,
-// loaded and stored one by one.
+// loaded and stored one by one.  The price against the vector kernels, at
+// 16384 x 2047 beside 2048: bf16 pack 33 us beside 20, unpack 41 / 19, swiglu8
+// forward 69 / 50, backward 79 / 51; fp32 37 / 29, 39 / 42, 87 / 77, 90 / 80.
 template <typename T>
 struct Four {
   float f[4];
@@ -440,9 +442,10 @@ swiglu8_bwd_any_kernel(const T* __restrict__ dh, const unsigned* __restrict__ co
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Grids of 256-thread blocks that loop, at most 16 a SM: swiglu8_fwd of 4096 x
-// 14336 took 76 us with 16, 77 with 8, 79 with the 4 that are resident at once,
-// 96 with 5 (a short second wave), and swiglu8_bwd 80 without a loop.
+// Grids of 256-thread blocks that loop, at most 16 a SM: calls of swiglu8_fwd at
+// 4096 x 14336 bf16 took 78 us each with 16, 80 with 8, 82 with the 4 that are
+// resident at once, 99 with 5 (a short second wave), and swiglu8_bwd 82, 87
+// without a loop.
 int loop_grid(long long threads) { return grid_for(threads, kThreads, kNumSMs * 16); }
 
 // f(first row, rows, threads' units of work) over parts of at most 2^30 units

@@ -801,10 +801,12 @@ def scaled_embedding(idx: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
                      padding_idx: Optional[int] = None) -> torch.Tensor:
     """``weight[idx] * scale`` for int64 ``idx`` of any shape and a [V, C] table.
 
-    The gradient of a row is the fp32 sum over its positions in ascending
-    order, rounded once, whatever runs beside it: the same from run to run
+    The gradient of a row is an fp32 sum over its positions, rounded once, in
+    an order that depends on the call's tokens alone: the same from run to run
     (:func:`embedding` adds with atomics, and keeps an fp32 [V, C] accumulator,
-    which this does not).  It goes into ``weight.grad`` where the engine has
+    which this does not).  On CUDA the order is that of the positions within
+    parts of the batch sorted by token, and then that of the parts; other
+    tokens in the batch move the cuts, and with them last bits.  It goes into ``weight.grad`` where the engine has
     bound one.  Positions equal to ``padding_idx`` give no gradient.
 
     A token outside the table raises ``IndexError`` on the CPU; on CUDA it

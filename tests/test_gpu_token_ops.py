@@ -361,7 +361,7 @@ def test_embedding_beyond_32_bit_offsets():
 
 
 def test_embedding_lookup_of_more_than_2_31_values():
-    """Places behind the end of a launch's last round, whose number times eight
+    """Places behind the end, in the last turn of a launch, whose number times eight
     passes 31 bits, read nothing."""
     n, V, C = 600001, 37, 4096
     w = _randn(V, C, dtype=torch.bfloat16)
